@@ -1,0 +1,686 @@
+"""Operators of long and branching generations over the paged KV cache, as cases
+that can be timed, each beside its plain form in elementary torch operations.
+
+* ``decode``: one new token per sequence that sees a sliding window of the
+  newest tokens and the first few (attention sinks), over the paged pool.
+  ``fused``: RoPE and the page append of the new rows run in the same call.
+* ``prefill``: a chunk of new tokens per sequence over a cached prefix, causal,
+  with the same window and sinks.
+* ``axes``: rotary positions with several axes (time, height, width) of the new
+  q and k rows, and the page append of the k and v rows.
+* ``upkeep``: what a step does to the page tables on the device: pages for the
+  new tokens, copy-on-write forks of shared partial pages, and the release of
+  the pages that fell out of the window.
+* ``compact``: the live pages of a scattered pool moved to its front, with the
+  page tables that name them.
+
+Head shapes are those of the repository's workloads: TinyLlama (32 query / 4
+KV heads, head_dim 64), Llama-3-8B (32 / 8, 128), a 70B-shaped layer (64 / 8,
+128) and that layer's share at tensor parallelism 8 (8 / 1, 128).  Pages are
+scattered over the pool.  Lengths belong to the case (``lens`` seeds them);
+values and page tables come from the run's seed.  A window of W sees the W
+tokens before a token and the token itself.
+"""
+
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+PAGE = 16
+THETA = 500000.0
+WORKSPACE = 128 * 1024 * 1024  # what the engine allocates
+HEADS = {"tinyllama": (32, 4, 64), "llama3_8b": (32, 8, 128), "70b": (64, 8, 128),
+         "70b_tp8": (8, 1, 128)}
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "e4m3": torch.bfloat16}
+DEV = "cuda"
+I32 = torch.int32
+
+
+def _kernels():
+    """The framework's package."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "llm-inference-runtime_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import pagedattn
+
+    return pagedattn
+
+
+# -- the cases ----------------------------------------------------------------
+
+def _decode(model, dtype, batch, lo, hi, window, sinks, lens, fused):
+    return {"op": "decode", "model": model, "dtype": dtype, "batch": batch, "lo": lo, "hi": hi,
+            "window": window, "sinks": sinks, "lens": lens, "fused": fused}
+
+
+def _prefill(model, dtype, batch, chunk_lo, chunk_hi, lo, hi, window, sinks, lens):
+    return {"op": "prefill", "model": model, "dtype": dtype, "batch": batch, "chunk_lo": chunk_lo,
+            "chunk_hi": chunk_hi, "lo": lo, "hi": hi, "window": window, "sinks": sinks,
+            "lens": lens}
+
+
+def _axes(model, dtype, batch, lo, hi, cyclic, lens):
+    return {"op": "axes", "model": model, "dtype": dtype, "batch": batch, "lo": lo, "hi": hi,
+            "cyclic": cyclic, "lens": lens}
+
+
+def _upkeep(model, dtype, batch, layers, pages, lo, hi, chunk, window, sinks, lens):
+    return {"op": "upkeep", "model": model, "dtype": dtype, "batch": batch, "layers": layers,
+            "pages": pages, "lo": lo, "hi": hi, "chunk": chunk, "window": window, "sinks": sinks,
+            "lens": lens}
+
+
+def _compact(model, dtype, batch, layers, pages, live, lens):
+    return {"op": "compact", "model": model, "dtype": dtype, "batch": batch, "layers": layers,
+            "pages": pages, "live": live, "lens": lens}
+
+
+def listed():
+    named = [
+        # a few chats on the engine's default model: the smallest decode step
+        ("decode_tinyllama_b4", _decode("tinyllama", "fp16", 4, 200, 6000, 1023, 4, 1, False)),
+        # an ordinary serving batch of long chats: RoPE, append and attention in one call
+        ("decode_llama3_8b_b64", _decode("llama3_8b", "bf16", 64, 1000, 60000, 4095, 4, 2, True)),
+        # a large model's full batch over an e4m3 pool: the most bytes of a step
+        ("decode_70b_e4m3_b128", _decode("70b", "e4m3", 128, 2000, 90000, 8191, 64, 3, False)),
+        # short prompts and chat turns that arrive together
+        ("prefill_tinyllama_prompts", _prefill("tinyllama", "fp16", 3, 90, 210, 0, 700, 255, 4, 4)),
+        # the next 512-token chunk (the engine's default step) of a long document, e4m3 pool
+        ("prefill_llama3_8b_e4m3_chunk",
+         _prefill("llama3_8b", "e4m3", 1, 512, 512, 20000, 20000, 4095, 4, 5)),
+        # whole prompts of thousands of tokens in one step: the most operations
+        ("prefill_llama3_8b_long",
+         _prefill("llama3_8b", "bf16", 2, 6000, 8192, 0, 0, 1023, 16, 6)),
+        # a decode step's rows of a model that also reads images
+        ("axes_tinyllama_b33", _axes("tinyllama", "fp16", 33, 1, 1, True, 7)),
+        # prompts of images and text
+        ("axes_llama3_8b_prompts", _axes("llama3_8b", "bf16", 4, 3000, 6000, False, 8)),
+        # page upkeep of a small decode batch
+        ("upkeep_tinyllama_b32",
+         _upkeep("tinyllama", "fp16", 32, 4, 4000, 200, 2500, 1, 1023, 4, 9)),
+        # decode rows and prompt chunks of a full batch over a pool of many pages
+        ("upkeep_70b_tp8_b512",
+         _upkeep("70b_tp8", "bf16", 512, 2, 100000, 500, 4000, 512, 2047, 64, 10)),
+        # a small pool whose long requests have ended
+        ("compact_tinyllama", _compact("tinyllama", "fp16", 24, 22, 1500, 0.3, 11)),
+        # a large one
+        ("compact_llama3_8b_e4m3", _compact("llama3_8b", "e4m3", 300, 4, 20000, 0.45, 12)),
+    ]
+    return [dict(c, name=n) for n, c in named]
+
+
+def _spread(rng, lo, hi):
+    """A whole number, spread over the logarithm of [lo, hi]."""
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    model = rng.choice(sorted(HEADS))
+    dtype = rng.choice(["bf16", "fp16", "e4m3"])
+    hq, hkv, d = HEADS[model]
+    lens = rng.randrange(1 << 20)
+    sinks = rng.choice([0, 1, 4, 16, rng.randrange(5, 200)])
+    window = rng.choice([127, 1023, 4095, _spread(rng, 16, 8192)])
+    op = rng.choice(["decode", "decode", "prefill", "prefill", "axes", "upkeep", "compact"])
+    if op == "decode":
+        row = (window + sinks) * hkv * d * (1 if dtype == "e4m3" else 2) * 2
+        batch = _spread(rng, 1, max(2, min(400, int(1.6e9) // row)))
+        lo = _spread(rng, 1, 20000)
+        fused = dtype != "e4m3" and rng.random() < 0.5
+        return _decode(model, dtype, batch, lo, lo + _spread(rng, 1, 60000), window, sinks, lens,
+                       fused)
+    if op == "prefill":
+        batch = _spread(rng, 1, 8)
+        chunk = _spread(rng, 2, max(3, 4096 // batch))
+        hi = rng.choice([0, _spread(rng, 1, 6000)])
+        return _prefill(model, dtype, batch, max(1, chunk // 2), chunk, 0, hi, window, sinks, lens)
+    if op == "axes":
+        batch = _spread(rng, 1, 64)
+        chunk = rng.choice([1, _spread(rng, 2, max(3, 16000 // batch))])
+        return _axes(model, dtype, batch, max(1, chunk // 2), chunk, rng.random() < 0.5, lens)
+    if op == "upkeep":
+        hi = _spread(rng, 20, 3000)
+        most = int(1.6e9) // (2 * hkv * PAGE * d * 2) - 20000 if hkv == 1 else 16000
+        batch = _spread(rng, 1, min(512, most // (hi // PAGE + 40)))
+        pages = batch * (hi // PAGE + 40) + rng.randrange(100, 6000)
+        return _upkeep(model, dtype, batch, 1, pages, max(1, hi // 3), hi,
+                       rng.choice([1, _spread(rng, 2, 512)]), window, sinks, lens)
+    layers = rng.choice([1, 2, 3])
+    pages = _spread(rng, 100, int(1.2e9) // (layers * 2 * hkv * PAGE * d * 2))
+    return _compact(model, dtype, rng.randrange(1, 200), layers, pages,
+                    round(rng.uniform(0.05, 0.95), 2), lens)
+
+
+# -- inputs -------------------------------------------------------------------
+
+def _lengths(case, n, lo, hi):
+    """n lengths spread over the logarithm of [lo, hi], the same for every seed."""
+    r = np.random.RandomState(case["lens"] % (1 << 31))
+    a, b = math.log(max(lo, 1)), math.log(max(hi, 1))
+    x = np.rint(np.exp(r.uniform(a, b, n))).astype(np.int64)
+    return np.clip(x, lo, hi) if lo > 0 else np.where(r.uniform(size=n) < 0.25, 0, x.clip(0, hi))
+
+
+def _rng(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(int(seed))
+    return g
+
+
+def _randn(shape, g, dtype):
+    return torch.randn(shape, generator=g, device=DEV, dtype=torch.float32).to(dtype)
+
+
+def _pool(shape, dtype, g):
+    """A pool of rows and, for e4m3, the scales of its (page, K|V, head) blocks."""
+    x = torch.empty(shape, dtype=DTYPES[dtype], device=DEV).normal_(generator=g)
+    if dtype != "e4m3":
+        return x, None
+    amax = x.abs().amax(dim=(-2, -1)).float()
+    scales = (amax / 448).clamp_min(1e-6)
+    return (x / scales[..., None, None]).to(torch.float8_e4m3fn), scales
+
+
+def _i32(a):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV)
+
+
+def _pages_of(n):
+    return -(-n // PAGE)
+
+
+def _paged(case, seed, kv_lens, first_seen):
+    """Page lists of sequences of kv_lens tokens: pages from the sinks to the one that holds
+    token first_seen[b] have been released (-1)."""
+    r = np.random.RandomState((seed * 7919 + 11) % (1 << 31))
+    counts = _pages_of(kv_lens)
+    indptr = np.concatenate([[0], np.cumsum(counts)])
+    slot = np.arange(indptr[-1]) - np.repeat(indptr[:-1], counts)
+    gone = (slot >= _pages_of(np.int64(case["sinks"]))) & \
+        (slot < np.repeat(np.maximum(first_seen, 0) // PAGE, counts))
+    n_live = int((~gone).sum())
+    num_pages = n_live + 8
+    indices = np.full(indptr[-1], -1, np.int64)
+    indices[~gone] = r.permutation(num_pages)[:n_live]
+    return {"kv_indptr": _i32(indptr), "kv_indices": _i32(indices),
+            "kv_last_page_len": _i32((kv_lens - 1) % PAGE + 1), "num_pages": num_pages}
+
+
+def _attention_state(case, seed):
+    hq, hkv, d = HEADS[case["model"]]
+    dt = DTYPES[case["dtype"]]
+    g = _rng(seed)
+    n = case["batch"]
+    if case["op"] == "decode":
+        chunk = np.ones(n, np.int64)
+        kv = np.maximum(_lengths(case, n, case["lo"], case["hi"]), 1)
+    else:
+        chunk = _lengths(case, n, case["chunk_lo"], case["chunk_hi"])
+        kv = chunk + _lengths(dict(case, lens=case["lens"] + 1), n, case["lo"], case["hi"])
+    s = _paged(case, seed, kv, kv - chunk - case["window"])
+    rows = int(chunk.sum())
+    # q, k and v rows are views of the projection's fused rows
+    qkv = _randn((rows, hq + 2 * hkv, d), g, dt)
+    s["q"], s["k"], s["v"] = qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    s["pool"], s["scales"] = _pool((s["num_pages"], 2, hkv, PAGE, d), case["dtype"], g)
+    s["qo_indptr"] = _i32(np.concatenate([[0], np.cumsum(chunk)]))
+    s["kv_lens"], s["chunk"] = _i32(kv), _i32(chunk)
+    s["kv_max"], s["chunk_max"] = int(kv.max()), int(chunk.max())
+    s["workspace"] = torch.zeros(WORKSPACE, dtype=torch.uint8, device=DEV)
+    return s
+
+
+def _sections(d, cyclic):
+    """Frequencies of the time, height and width axes."""
+    f = d // 2
+    side = f // 3 if cyclic else 3 * f // 8
+    return (f - 2 * side, side, side)
+
+
+def _axes_state(case, seed):
+    hq, hkv, d = HEADS[case["model"]]
+    dt = DTYPES[case["dtype"]]
+    g = _rng(seed)
+    n = case["batch"]
+    chunk = _lengths(case, n, case["lo"], case["hi"])
+    prefix = np.random.RandomState(case["lens"] % (1 << 31)).randint(0, 2000, n)
+    kv = chunk + prefix
+    s = _paged(dict(case, sinks=0), seed, kv, prefix // PAGE * PAGE)
+    rows = int(chunk.sum())
+    qkv = _randn((rows, hq + 2 * hkv, d), g, dt)
+    s["q"], s["k"], s["v"] = qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    s["pool"], s["scales"] = _pool((s["num_pages"], 2, hkv, PAGE, d), case["dtype"], g)
+    within = np.arange(rows) - np.repeat(np.cumsum(chunk) - chunk, chunk)
+    s["batch_indices"] = _i32(np.repeat(np.arange(n), chunk))
+    s["positions"] = _i32(np.repeat(prefix, chunk) + within)
+    # spans of 256 tokens, text and images of 16 x 16 patches in turn
+    start, image = within // 256 * 256, within // 256 % 2 == 1
+    base = np.repeat(prefix, chunk) + start
+    s["axis_positions"] = _i32(np.stack([
+        base + np.where(image, 0, within - start),
+        base + np.where(image, (within - start) // 16, within - start),
+        base + np.where(image, (within - start) % 16, within - start)]))
+    s["sections"] = _sections(d, case["cyclic"])
+    return s
+
+
+def _tables_state(case, seed):
+    """Page tables, reference counts and the whole pool of all layers."""
+    hq, hkv, d = HEADS[case["model"]]
+    g = _rng(seed)
+    r = np.random.RandomState((seed * 7919 + 13) % (1 << 31))
+    n, num_pages = case["batch"], case["pages"]
+    s = {}
+    s["pool"], s["scales"] = _pool((case["layers"], num_pages, 2, hkv, PAGE, d), case["dtype"], g)
+    if case["op"] == "upkeep":
+        held = _lengths(case, n, case["lo"], case["hi"])
+        new = np.where(np.arange(n) % 8 == 3, case["chunk"], 1)
+        held[1::4] = held[0::4][:len(held[1::4])]  # second samples of one prompt
+        counts = _pages_of(held)
+        width = int(_pages_of(held + new).max()) + 3
+        s["kv_lens"], s["new_lens"] = _i32(held + new), _i32(new)
+    else:
+        r2 = np.random.RandomState(case["lens"] % (1 << 31))
+        live = max(1, int(case["live"] * num_pages))
+        counts = np.diff(np.concatenate([[0], np.sort(r2.randint(0, live + 1, n - 1)), [live]]))
+        width = int(counts.max()) + 1
+    order = r.permutation(num_pages)
+    starts = np.cumsum(counts) - counts
+    tables = np.full((n, width), -1, np.int64)
+    col = np.arange(width)[None, :]
+    inside = col < counts[:, None]
+    tables[inside] = order[(starts[:, None] + col)[inside] % num_pages]
+    if case["op"] == "upkeep":
+        tables[1::4] = tables[0::4][:len(tables[1::4])]
+    refs = np.bincount(tables[tables >= 0], minlength=num_pages)
+    s["block_tables"], s["ref_counts"] = _i32(tables), _i32(refs)
+    return s
+
+
+def prepare(case, seed):
+    if case["op"] in ("decode", "prefill"):
+        s = _attention_state(case, seed)
+    elif case["op"] == "axes":
+        s = _axes_state(case, seed)
+    else:
+        s = _tables_state(case, seed)
+    s["case"] = case
+    return s
+
+
+# -- plain forms --------------------------------------------------------------
+
+def _rows_of(s, page, slot, kind):
+    """The K (0) or V (1) rows at (page, slot) in 32 bits, [..., Hkv, D]."""
+    page = page.clamp_min(0).long()
+    x = s["pool"][page, kind, :, slot.long()].float()
+    return x if s["scales"] is None else x * s["scales"][page, kind][..., None]
+
+
+def _rotation(pos, d):
+    """cos and sin of position `pos` at every frequency, angles in 64 bits."""
+    inv = THETA ** (-torch.arange(0, d, 2, device=pos.device, dtype=torch.float64) / d)
+    ang = pos.double()[..., None] * inv
+    return torch.cos(ang).float(), torch.sin(ang).float()
+
+
+def _rotate(x, cos, sin):
+    """x [n, heads, d] rotated in 32 bits, pairs half a head apart."""
+    a, b = x.float().chunk(2, dim=-1)
+    cos, sin = cos[:, None], sin[:, None]
+    return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+
+
+def _softmax_rows(scores, v, seen):
+    """softmax of scores where `seen`, times v; and the log-sum-exp.  Rows that see nothing are
+    zero with -inf."""
+    scores = scores.masked_fill(~seen, -math.inf)
+    top = scores.amax(dim=-1, keepdim=True)
+    top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+    p = torch.exp(scores - top)
+    total = p.sum(dim=-1, keepdim=True)
+    out = torch.matmul(p, v) / torch.where(total > 0, total, torch.ones_like(total))
+    return out, (top + torch.log(total)).squeeze(-1)
+
+
+def _plain_decode(s, case):
+    hq, hkv, d = HEADS[case["model"]]
+    n = case["batch"]
+    lens = s["kv_lens"].long()
+    first = s["kv_indptr"][:-1].long()
+    if case["fused"]:
+        cos, sin = _rotation(lens - 1, d)
+        q, k = _rotate(s["q"], cos, sin), _rotate(s["k"], cos, sin).to(s["pool"].dtype)
+        page = s["kv_indices"][first + (lens - 1) // PAGE].long()
+        s["pool"][page, 0, :, (lens - 1) % PAGE] = k
+        s["pool"][page, 1, :, (lens - 1) % PAGE] = s["v"]
+    else:
+        q = s["q"].float()
+    # the sinks, then the window's tokens: absent ones are masked
+    start = torch.clamp(lens - 1 - case["window"], min=0)
+    sink = min(case["sinks"], s["kv_max"])
+    span = min(case["window"] + 1, s["kv_max"])
+    a = torch.arange(sink, device=DEV).expand(n, sink)
+    b = start[:, None] + torch.arange(span, device=DEV)
+    tok = torch.cat([a, b], dim=1)
+    seen = torch.cat([a < torch.minimum(start, lens)[:, None], b < lens[:, None]], dim=1)
+    tok = torch.minimum(tok, (lens - 1)[:, None])
+    page = s["kv_indices"][first[:, None] + tok // PAGE]
+    k = _rows_of(s, page, tok % PAGE, 0).transpose(1, 2)
+    v = _rows_of(s, page, tok % PAGE, 1).transpose(1, 2)
+    q = q.reshape(n, hkv, hq // hkv, d)
+    scores = torch.matmul(q, k.transpose(2, 3)) / math.sqrt(d)
+    out, lse = _softmax_rows(scores, v, seen[:, None, None])
+    out = out.reshape(n, hq, d).to(s["q"].dtype)
+    return {"out": out, "pool": s["pool"]} if case["fused"] else \
+        {"out": out, "lse": lse.reshape(n, hq)}
+
+
+def _plain_prefill(s, case):
+    hq, hkv, d = HEADS[case["model"]]
+    n, g = case["batch"], hq // hkv
+    lens, chunk = s["kv_lens"].long(), s["chunk"].long()
+    first = s["kv_indptr"][:-1].long()
+    row0 = s["qo_indptr"][:-1].long()
+    i = torch.arange(s["chunk_max"], device=DEV)
+    j = torch.arange(s["kv_max"], device=DEV)
+    valid = i < chunk[:, None]
+    rows = torch.where(valid, row0[:, None] + i, row0[:, None])
+    at = (lens - chunk)[:, None, None] + i[:, None]
+    seen = (j <= at) & ((j >= at - case["window"]) | (j < case["sinks"]))
+    tok = torch.minimum(j, (lens - 1)[:, None])
+    page = s["kv_indices"][first[:, None] + tok // PAGE]
+    k = _rows_of(s, page, tok % PAGE, 0).transpose(1, 2)
+    v = _rows_of(s, page, tok % PAGE, 1).transpose(1, 2)
+    q = s["q"][rows].float().reshape(n, -1, hkv, g, d).transpose(1, 2).reshape(n, hkv, -1, d)
+    scores = torch.matmul(q, k.transpose(2, 3)) / math.sqrt(d)
+    scores = scores.view(n, hkv, -1, g, s["kv_max"])
+    scores = scores.masked_fill(~seen[:, None, :, None], -math.inf).view(n, hkv, -1, s["kv_max"])
+    top = scores.amax(dim=-1, keepdim=True)
+    top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+    p = torch.exp(scores.sub_(top))
+    total = p.sum(dim=-1, keepdim=True)
+    out = torch.matmul(p, v) / total.clamp_min(1e-30)
+    lse = (top + torch.log(total)).view(n, hkv, -1, g).transpose(1, 2).reshape(n, -1, hq)
+    out = out.view(n, hkv, -1, g, d).transpose(1, 2).reshape(n, -1, hq, d)
+    # row r of the batch is row r - row0[b] of its sequence b
+    r = torch.arange(s["q"].shape[0], device=DEV)
+    b = torch.searchsorted(s["qo_indptr"][1:].long(), r, right=True)
+    return {"out": out[b, r - row0[b]].to(s["q"].dtype), "lse": lse[b, r - row0[b]]}
+
+
+def _axis_of(sections, cyclic):
+    """The axis whose position turns each frequency: blocks of frequencies, or the axes in turn
+    as far as their shares reach and the first axis beyond."""
+    f = torch.arange(sum(sections), device=DEV)
+    if not cyclic:
+        edges = torch.tensor(sections, device=DEV).cumsum(0)
+        return torch.searchsorted(edges, f, right=True)
+    turn = f % len(sections)
+    share = torch.tensor(sections, device=DEV)[turn] * len(sections)
+    return torch.where(f < share, turn, torch.zeros_like(turn))
+
+
+def _plain_axes(s, case):
+    d = HEADS[case["model"]][2]
+    axis = _axis_of(s["sections"], case["cyclic"])
+    pos = s["axis_positions"].long()[axis].T  # [n, d / 2]
+    inv = THETA ** (-torch.arange(0, d, 2, device=DEV, dtype=torch.float64) / d)
+    ang = pos.double() * inv
+    cos, sin = torch.cos(ang).float(), torch.sin(ang).float()
+    s["q"].copy_(_rotate(s["q"], cos, sin))
+    s["k"].copy_(_rotate(s["k"], cos, sin))
+    at = s["positions"].long()
+    page = s["kv_indices"][s["kv_indptr"][s["batch_indices"].long()].long() + at // PAGE].long()
+    k, v = s["k"], s["v"]
+    if s["scales"] is not None:
+        k = (k.float() / s["scales"][page, 0][..., None]).clamp(-448, 448)
+        v = (v.float() / s["scales"][page, 1][..., None]).clamp(-448, 448)
+    s["pool"][page, 0, :, at % PAGE] = k.to(s["pool"].dtype)
+    s["pool"][page, 1, :, at % PAGE] = v.to(s["pool"].dtype)
+    return {"q": s["q"], "k": s["k"], "pool": s["pool"]}
+
+
+def _plain_upkeep(s, case):
+    tables, refs = s["block_tables"].clone(), s["ref_counts"].clone()
+    pool, lens = s["pool"], s["kv_lens"].long()
+    n, width = tables.shape
+    held = lens - s["new_lens"]
+    first, last = (held + PAGE - 1) // PAGE, (lens + PAGE - 1) // PAGE
+    # a sequence forks the partial page it appends to while others hold it
+    row, spot = torch.arange(n, device=DEV), held // PAGE
+    shared = tables[row, spot.clamp_max(width - 1)].long()
+    part = (held % PAGE != 0) & (s["new_lens"] > 0)
+    same = (shared[:, None] == shared) & part & part[:, None]
+    earlier = torch.tril(same, diagonal=-1).sum(dim=1)
+    fork = part & (refs[shared.clamp_min(0)] - earlier > 1)
+    need = last - first + fork
+    base = torch.cumsum(need, 0) - need
+    # the free pages in order: those that no table names
+    free = torch.argsort((refs != 0).to(torch.uint8), stable=True)
+    col = torch.arange(width, device=DEV)
+    new = (col >= first[:, None]) & (col < last[:, None])
+    forked = fork[:, None] & (col == spot[:, None])
+    rank = torch.where(forked, base[:, None], (base + fork - first)[:, None] + col)
+    got = free[rank.clamp(0, free.numel() - 1)].to(I32)
+    took = new | forked
+    tables = torch.where(took, got, tables)
+    refs.index_add_(0, got.reshape(-1), took.reshape(-1).to(I32))
+    refs.index_add_(0, shared.clamp_min(0), -fork.to(I32))
+    who = torch.nonzero(fork).squeeze(1)
+    src, to = shared[who], tables[who, spot[who]].long()
+    keep = torch.arange(PAGE, device=DEV) < (held % PAGE)[who][:, None]
+    keep = keep[None, :, None, None, :, None]
+    bits = pool.view(torch.uint8 if s["scales"] is not None else torch.int16)
+    bits[:, to] = torch.where(keep, bits[:, src], bits[:, to])
+    if s["scales"] is not None:
+        s["scales"][:, to] = s["scales"][:, src]
+    # pages that the next token's window has left behind
+    lo = _pages_of(case["sinks"])
+    hi = torch.clamp(lens - 1 - case["window"], min=0) // PAGE
+    gone = (col >= lo) & (col < hi[:, None]) & (tables >= 0)
+    refs.index_add_(0, tables.clamp_min(0).reshape(-1), -gone.reshape(-1).to(I32))
+    tables = torch.where(gone, torch.full_like(tables, -1), tables)
+    return {"block_tables": tables, "ref_counts": refs, "pool": pool}
+
+
+def _plain_compact(s, case):
+    tables, refs = s["block_tables"].clone(), s["ref_counts"].clone()
+    pool = s["pool"]
+    page = torch.arange(refs.numel(), device=DEV)
+    live = refs > 0
+    line = live.sum()
+    src = torch.nonzero(live & (page >= line)).squeeze(1)
+    dst = torch.nonzero(~live & (page < line)).squeeze(1)
+    remap = torch.where(live, page, torch.full_like(page, -1)).to(I32)
+    remap[src] = dst.to(I32)
+    bits = pool.view(torch.uint8 if s["scales"] is not None else torch.int16)
+    bits[:, dst] = bits[:, src]
+    if s["scales"] is not None:
+        s["scales"][:, dst] = s["scales"][:, src]
+    refs[dst] = refs[src]
+    refs[src] = 0
+    tables = torch.where(tables >= 0, remap[tables.clamp_min(0).long()], tables)
+    return {"block_tables": tables, "ref_counts": refs, "remap": remap, "pool": pool}
+
+
+# -- the framework's calls ----------------------------------------------------
+
+def _own_decode(s, case):
+    pa = _kernels()
+    hq, hkv, d = HEADS[case["model"]]
+    w = pa.BatchDecodeWithPagedKVCacheWrapper(s["workspace"], "HND")
+    w.plan(s["kv_indptr"], s["kv_indices"], s["kv_last_page_len"], hq, hkv, d, PAGE,
+           q_data_type=s["q"].dtype, window_left=case["window"], num_sink_tokens=case["sinks"],
+           device_plan=True)
+    if case["fused"]:
+        out = w.run(s["q"], s["pool"], kv_scales=s["scales"], append_key=s["k"],
+                    append_value=s["v"], rope=(1.0, THETA))
+        return {"out": out, "pool": s["pool"]}
+    out, lse = w.run(s["q"], s["pool"], kv_scales=s["scales"], return_lse=True)
+    return {"out": out, "lse": lse}
+
+
+def _own_prefill(s, case):
+    pa = _kernels()
+    hq, hkv, d = HEADS[case["model"]]
+    w = pa.BatchPrefillWithPagedKVCacheWrapper(s["workspace"], "HND")
+    w.plan(s["qo_indptr"], s["kv_indptr"], s["kv_indices"], s["kv_last_page_len"], hq, hkv, d,
+           PAGE, causal=True, q_data_type=s["q"].dtype, window_left=case["window"],
+           num_sink_tokens=case["sinks"], device_plan=True, max_qo_tokens=s["q"].shape[0])
+    out, lse = w.run(s["q"], s["pool"], kv_scales=s["scales"], return_lse=True)
+    return {"out": out, "lse": lse}
+
+
+def _own_axes(s, case):
+    _kernels().multi_axis_rope_append_paged_kv_cache(
+        s["q"], s["k"], s["v"], s["axis_positions"], s["sections"], s["batch_indices"],
+        s["positions"], s["pool"], s["kv_indices"], s["kv_indptr"], s["kv_last_page_len"],
+        kv_layout="HND", rope_theta=THETA, cyclic=case["cyclic"], kv_scales=s["scales"])
+    return {"q": s["q"], "k": s["k"], "pool": s["pool"]}
+
+
+def _own_upkeep(s, case):
+    pa = _kernels()
+    tables, refs = s["block_tables"].clone(), s["ref_counts"].clone()
+    pa.reserve_pages(s["pool"], tables, s["kv_lens"], s["new_lens"], refs, kv_scales=s["scales"])
+    pa.release_window_pages(tables, s["kv_lens"], refs, window_left=case["window"],
+                            num_sink_tokens=case["sinks"])
+    return {"block_tables": tables, "ref_counts": refs, "pool": s["pool"]}
+
+
+def _own_compact(s, case):
+    tables, refs = s["block_tables"].clone(), s["ref_counts"].clone()
+    remap = _kernels().compact_pages(s["pool"], tables, refs, kv_scales=s["scales"])
+    return {"block_tables": tables, "ref_counts": refs, "remap": remap, "pool": s["pool"]}
+
+
+def run(state):
+    case = state["case"]
+    op = case["op"]
+    if own:
+        return {"decode": _own_decode, "prefill": _own_prefill, "axes": _own_axes,
+                "upkeep": _own_upkeep, "compact": _own_compact}[op](state, case)
+    return {"decode": _plain_decode, "prefill": _plain_prefill, "axes": _plain_axes,
+            "upkeep": _plain_upkeep, "compact": _plain_compact}[op](state, case)
+
+
+# -- what a pass cannot do without -------------------------------------------
+
+def work(case):
+    hq, hkv, d = HEADS[case["model"]]
+    size = 1 if case["dtype"] == "e4m3" else 2
+    n, op = case["batch"], case["op"]
+    if op in ("decode", "prefill"):
+        if op == "decode":
+            chunk = np.ones(n, np.int64)
+            kv = np.maximum(_lengths(case, n, case["lo"], case["hi"]), 1)
+        else:
+            chunk = _lengths(case, n, case["chunk_lo"], case["chunk_hi"])
+            kv = chunk + _lengths(dict(case, lens=case["lens"] + 1), n, case["lo"], case["hi"])
+        seen, read = 0, 0
+        for c, length in zip(chunk.tolist(), kv.tolist()):
+            at = np.arange(length - c, length)
+            start = np.maximum(at - case["window"], 0)
+            seen += int((at + 1 - start + np.minimum(start, case["sinks"])).sum())
+            read += length - int(start[0]) + min(int(start[0]), case["sinks"])
+        rows = int(chunk.sum())
+        total = 2 * read * hkv * d * size + 2 * rows * hq * d * 2
+        if op == "decode" and case["fused"]:
+            total += rows * hkv * d * 4 * 2
+        return {"bytes": total, "flops": 4 * d * hq * seen}
+    if op == "axes":
+        rows = int(_lengths(case, n, case["lo"], case["hi"]).sum())
+        return {"bytes": rows * d * (2 * 2 * (hq + hkv) + 2 * hkv + 2 * hkv * size),
+                "flops": 3 * rows * d * (hq + hkv)}
+    page = case["layers"] * 2 * hkv * (PAGE * d * size + (4 if size == 1 else 0))
+    if op == "upkeep":
+        held = _lengths(case, n, case["lo"], case["hi"])
+        held[1::4] = held[0::4][:len(held[1::4])]
+        forks = int((held[1::4] % PAGE != 0).sum())
+        width = int(_pages_of(held + np.where(np.arange(n) % 8 == 3, case["chunk"], 1)).max()) + 3
+        return {"bytes": 4 * (case["pages"] + n * width) + forks * page, "flops": 0}
+    # the moves of a scattered pool: live pages above the line, which are its holes below
+    moved = case["live"] * (1 - case["live"]) * case["pages"]
+    return {"bytes": int(2 * moved * page) + 12 * case["pages"], "flops": 0}
+
+
+# -- the definition in 64 bits ------------------------------------------------
+
+def _exact_attention(s, case):
+    hq, hkv, d = HEADS[case["model"]]
+    g = hq // hkv
+    indptr, qo = s["kv_indptr"].tolist(), s["qo_indptr"].tolist()
+    kv_lens = s["kv_lens"].tolist()
+    out = torch.zeros(s["q"].shape, dtype=torch.float64, device=DEV)
+    lse = torch.zeros(s["q"].shape[:2], dtype=torch.float64, device=DEV)
+    freq = torch.exp(-math.log(THETA) / (d // 2) *
+                     torch.arange(d // 2, device=DEV, dtype=torch.float64))
+    for b, length in enumerate(kv_lens):
+        rows = slice(qo[b], qo[b + 1])
+        m = qo[b + 1] - qo[b]
+        ids = s["kv_indices"][indptr[b]:indptr[b + 1]].long()
+        live = torch.nonzero(ids >= 0).squeeze(1)
+        kv = s["pool"][ids[live]].double()
+        if s["scales"] is not None:
+            kv = kv * s["scales"][ids[live]].double()[..., None, None]
+        place = (live[:, None] * PAGE + torch.arange(PAGE, device=DEV)).reshape(-1)
+        k = kv[:, 0].transpose(0, 1).reshape(hkv, -1, d)
+        v = kv[:, 1].transpose(0, 1).reshape(hkv, -1, d)
+        q = s["q"][rows].double()
+        if case.get("fused"):
+            ang = (length - 1) * freq
+            turn = torch.polar(torch.ones_like(ang), ang)
+            q = torch.complex(q[..., :d // 2], q[..., d // 2:]) * turn
+            q = torch.cat([q.real, q.imag], dim=-1)
+            new = s["k"][rows].double()[0]
+            new = torch.complex(new[:, :d // 2], new[:, d // 2:]) * turn
+            newest = place == length - 1
+            k[:, newest] = torch.cat([new.real, new.imag], dim=-1)[:, None]
+            v[:, newest] = s["v"][rows].double()[0][:, None]
+        at = torch.arange(length - m, length, device=DEV)[:, None]
+        hidden = (place > at) | ((place < at - case["window"]) & (place >= case["sinks"]))
+        for h in range(hkv):
+            x = q[:, h * g:(h + 1) * g].reshape(m * g, d) @ k[h].T * d ** -0.5
+            x = x.view(m, g, -1).masked_fill(hidden[:, None], -math.inf)
+            total = torch.logsumexp(x, dim=-1)
+            p = torch.exp(x - total[..., None]).view(m * g, -1)
+            out[rows, h * g:(h + 1) * g] = (p @ v[h]).view(m, g, d)
+            lse[rows, h * g:(h + 1) * g] = total
+    return {"out": out, "pool": None} if case.get("fused") else {"out": out, "lse": lse}
+
+
+def _exact_axes(s, case):
+    d = HEADS[case["model"]][2]
+    f = d // 2
+    names, sections = [], s["sections"]
+    for a, count in enumerate(sections):
+        names += [a] * count
+    if case["cyclic"]:
+        names = [0] * f
+        for a in range(1, len(sections)):
+            for k in range(sections[a]):
+                names[len(sections) * k + a] = a
+    freq = [THETA ** (-2.0 * i / d) for i in range(f)]
+    ang = s["axis_positions"].double()[names].T * torch.tensor(freq, dtype=torch.float64,
+                                                                device=DEV)
+    turn = torch.polar(torch.ones_like(ang), ang)[:, None]
+    got = []
+    for x in (s["q"].double(), s["k"].double()):
+        y = torch.complex(x[..., :f], x[..., f:]) * turn
+        got.append(torch.cat([y.real, y.imag], dim=-1))
+    return {"q": got[0], "k": got[1], "pool": None}
+
+
+def exact(case, seed):
+    """None for page upkeep, whose outputs are whole numbers and copied pages."""
+    if case["op"] in ("upkeep", "compact"):
+        return None
+    s = prepare(case, seed)
+    return _exact_axes(s, case) if case["op"] == "axes" else _exact_attention(s, case)
