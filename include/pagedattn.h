@@ -428,6 +428,61 @@ int pagedattn_decode_run_scratch(
     float* lse, float sm_scale, void* scratch, size_t scratch_bytes,
     void* stream);
 
+/* Sliding window with sinks.  A token at position p sees the positions j <= p
+ * with j >= p - window_left or j < sinks (window_left -1: all of them).  Pages
+ * that no token of a call sees are not read, so their entries may name any page
+ * or none (-1).  A row's result does not depend on what tokens it does not see
+ * hold, infinities and NaN included.
+ *
+ * Decode works on lists of the visible pages.  pagedattn_decode_window_metadata
+ * makes them (device, graph-capturable, one launch): out_indptr [batch_size + 1],
+ * out_indices [out_capacity; ceil(sinks / 16) + window_left / 16 + 2 entries per
+ * sequence hold any step], holes [batch_size, 4] = {first and end of the unseen
+ * tokens around the seam, in tokens of the listed pages; pages left out; sink
+ * pages}.  pagedattn_decode_plan_window is pagedattn_decode_plan for the lists of
+ * a step whose host metadata is given; pagedattn_decode_plan_device needs
+ * no other form.  pagedattn_decode_run_window is pagedattn_decode_run_scratch over
+ * the lists (kv_indices, num_indices and kv_indptr are theirs); holes NULL
+ * is that call.  positions are those of the sequences. */
+int pagedattn_decode_window_metadata(const int32_t* kv_indptr, const int32_t* kv_indices,
+                                     int32_t num_indices, const int32_t* kv_last_page_len,
+                                     int32_t batch_size, int32_t window_left, int32_t sinks,
+                                     int32_t* out_indptr, int32_t* out_indices,
+                                     int32_t out_capacity, int32_t* holes, void* stream);
+int pagedattn_decode_plan_window(pagedattn_plan* plan, const int32_t* kv_indptr_host,
+                                 const int32_t* kv_last_page_len_host, int32_t batch_size,
+                                 int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t page_size, int32_t split_pages, int32_t window_left,
+                                 int32_t sinks, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+int pagedattn_decode_run_window(
+    const pagedattn_plan* plan, const int32_t* holes, const void* q, int64_t q_stride_n,
+    int64_t q_stride_h, int32_t q_dtype, const void* append_key,
+    const void* append_value, int64_t k_stride_n, int64_t k_stride_h,
+    int64_t v_stride_n, int64_t v_stride_h, int32_t rope,
+    const int32_t* positions, float rope_scale, float rope_theta,
+    void* paged_kv_cache, int32_t kv_dtype, const float* kv_scales,
+    int32_t num_pages, const int32_t* kv_indices, int32_t num_indices,
+    const int32_t* kv_indptr, const int32_t* kv_last_page_len, void* out,
+    float* lse, float sm_scale, void* scratch, size_t scratch_bytes,
+    void* stream);
+
+/* Prefill takes the window with its plan: pagedattn_prefill_plan and
+ * pagedattn_prefill_plan_device whose runs are windowed. */
+int pagedattn_prefill_plan_window(pagedattn_plan* plan, const int32_t* qo_indptr_host,
+                                  const int32_t* kv_indptr_host,
+                                  const int32_t* kv_last_page_len_host,
+                                  int32_t batch_size, int32_t num_qo_heads,
+                                  int32_t num_kv_heads, int32_t head_dim,
+                                  int32_t page_size, int32_t window_left, int32_t sinks,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+int pagedattn_prefill_plan_device_window(pagedattn_plan* plan, int32_t batch_size,
+                                         int32_t num_qo_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, int32_t page_size,
+                                         int64_t max_qo_tokens, int32_t window_left,
+                                         int32_t sinks, void* workspace,
+                                         size_t workspace_bytes);
+
 /* BatchPrefillWithPagedKVCacheWrapper.begin_forward(qo_indptr, kv_indptr,
  *     kv_indices, kv_last_page_len, Hq, Hkv, D, page_size, q_data_type)
  *     (src/models/llama.py:86-116).  Host copies of the indptr arrays.

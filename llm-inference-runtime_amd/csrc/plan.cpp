@@ -43,6 +43,15 @@ int validate_paged_metadata(const char* who, const int32_t* kv_indptr_host,
   return PAGEDATTN_OK;
 }
 
+int check_window(const char* who, int32_t window_left, int32_t sinks) {
+  if (window_left < -1 || sinks < 0 || (window_left < 0 && sinks > 0))
+    return set_error(PAGEDATTN_ERR_INVALID,
+                     "%s: window_left %d with %d sink tokens (a window is 0 or more, -1 for "
+                     "none, which has no sinks)",
+                     who, window_left, sinks);
+  return PAGEDATTN_OK;
+}
+
 int validate_heads(const char* who, int32_t hq, int32_t hkv, int32_t d,
                    int32_t page_size) {
   if (page_size != kPage)

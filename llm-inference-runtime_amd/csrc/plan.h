@@ -119,6 +119,44 @@ inline __host__ __device__ bool prefill_split_pays(int t_max, int len, int64_t c
   return t_max - len >= 4 && cost < 3 * slots * t_max;
 }
 
+// Sliding window with sinks: a token at position p sees positions j <= p with
+// j >= p - window_left or j < sinks.  The KV tiles that some of the tokens from
+// position p_lo on see, up to kv_end: [0, sink_tiles) and [first, end), `total`
+// in all.  A run's tile t of these is KV tile t, or first + t - sink_tiles.
+struct WindowTiles {
+  int sink_tiles, first, total;
+};
+inline __host__ __device__ WindowTiles window_tiles(int64_t kv_end, int64_t p_lo, int window_left,
+                                                    int sinks) {
+  const int n = (int)((kv_end + kPrefillKvTile - 1) / kPrefillKvTile);
+  const int64_t start = p_lo > window_left ? p_lo - window_left : 0;
+  const int64_t sink = sinks < kv_end ? sinks : kv_end;
+  const int st = (int)((sink + kPrefillKvTile - 1) / kPrefillKvTile);
+  int64_t first = start / kPrefillKvTile;
+  if (first > n) first = n;
+  if (first < st) first = st;
+  return WindowTiles{st, (int)first, st + n - (int)first};
+}
+
+// The pages of a decode step's sequence of `npages` pages, the last holding
+// `last` tokens, that its newest token sees: `npages` listed ones, those of the
+// sinks and those from the window's start on, with a hole [hole_lo, hole_hi) of
+// unseen tokens (counted in listed pages) around the seam.  A listed page at or
+// past `sink_pages` is page + shift of the sequence.
+struct WindowPages {
+  int npages, hole_lo, hole_hi, shift, sink_pages;
+};
+inline __host__ __device__ WindowPages window_pages(int npages, int last, int window_left,
+                                                    int sinks) {
+  const int64_t len = npages > 0 ? (int64_t)(npages - 1) * kPage + last : 0;
+  const int64_t start = len - 1 - window_left;
+  if (start <= sinks) return WindowPages{npages, 0, 0, 0, 0};
+  const int sp = (int)(((int64_t)sinks + kPage - 1) / kPage);
+  const int wp = (int)(start / kPage);
+  const int shift = wp > sp ? wp - sp : 0;
+  return WindowPages{npages - shift, sinks, (int)(start - (int64_t)kPage * shift), shift, sp};
+}
+
 // Workspace of a prefill plan that may cut tiles, from the workspace start: the
 // `tiles` whole tiles, the cut tiles' count, `entries` pieces and the merge list
 // of at most `slots` pieces per KV head.
@@ -182,6 +220,8 @@ struct pagedattn_plan {
   bool dev_table = false;
   // prefill: query tokens per tile (rows = tokens * hq/hkv)
   int q_tile = 0;
+  // prefill: the window's tokens before a token (-1: no window), and the sinks
+  int window_left = -1, sinks = 0;
   // prefill: tiles of at most half a workgroup's rows run as KV-head pairs
   // (device plans apply it at run time; host plans flag their items)
   bool prefill_pair = false;

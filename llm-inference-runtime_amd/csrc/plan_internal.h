@@ -15,6 +15,9 @@ int validate_paged_metadata(const char* who, const int32_t* kv_indptr_host,
                             std::vector<int32_t>* npages,
                             std::vector<int32_t>* kv_len);
 
+// Checks a sliding window (window_left -1: none, without sinks).
+int check_window(const char* who, int32_t window_left, int32_t sinks);
+
 // Checks the head shape the kernels support.
 int validate_heads(const char* who, int32_t hq, int32_t hkv, int32_t d,
                    int32_t page_size);

@@ -65,6 +65,7 @@ struct PrefillParams {
   float* partial_o;
   float* partial_lse;
   int32_t n_slots;
+  int32_t window_left, sinks;  // WINDOW (window_tiles in plan.h)
 };
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -168,6 +169,17 @@ __device__ __forceinline__ int fetch_page_ids(const PrefillParams& p,
   int id = -1;
   if (lane < 4 && pg < npages && ind_lo >= 0 && ind_lo + pg < p.num_indices)
     id = p.kv_indices[ind_lo + pg];
+  return id;
+}
+// Windowed tiles: pages [dead_lo, dead_hi) count as absent.
+template <bool WINDOW>
+__device__ __forceinline__ int fetch_seen_ids(const PrefillParams& p, int ind_lo, int npages,
+                                              int tile, int lane, int dead_lo, int dead_hi) {
+  const int id = fetch_page_ids(p, ind_lo, npages, tile, lane);
+  if constexpr (WINDOW) {
+    const int pg = tile * 4 + lane;
+    if (pg >= dead_lo && pg < dead_hi) return -1;
+  }
   return id;
 }
 
@@ -281,7 +293,83 @@ __device__ __forceinline__ float lane_value(float v, int i) {
 // rescale of O and l runs on few tiles.
 constexpr float kRescaleSlack = 8.f;
 
-template <int D, bool BF16, bool FP8, int RB, bool SPLIT>
+// One row of a windowed tile, element by element: what prefill_kernel computes
+// for the tokens of KV tiles [t_lo, t_hi) that the row at position `pos` sees,
+// by all 64 lanes of a wave (lane -> token, then lane -> d).  Called for rows
+// that came out not finite only: a tile's V rows are multiplied for every row
+// of the tile, by a weight of 0 where a row does not see the token, and 0 times an
+// infinity or a NaN that other rows see, or none does, is NaN.  o[e] is element
+// lane D / 64 + e of the row.
+template <int D, bool BF16, bool FP8>
+__device__ __forceinline__ void window_row(const PrefillParams& p, int h, int ind_lo, int npages,
+                                           int kv_len, int pos, int lim, WindowTiles wt, int t_lo,
+                                           int t_hi, const uint16_t* q, int lane,
+                                           float (&o)[D / kWave], float* m_out, float* l_out) {
+  constexpr int E = D / kWave;
+  constexpr int ESZ = FP8 ? 1 : 2;
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  auto value = [](const uint8_t* x) {
+    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8((int)*x, 0);
+    else return h2f<BF16>(*reinterpret_cast<const uint16_t*>(x));
+  };
+  for (int t = t_lo; t < t_hi; ++t) {
+    const int kt = t < wt.sink_tiles ? t : t - wt.sink_tiles + wt.first;
+    const int tok = kt * kPrefillKvTile + lane;
+    const bool seen = tok < kv_len && tok <= lim &&
+                      ((int64_t)tok >= (int64_t)pos - p.window_left || tok < p.sinks);
+    int page = -1;
+    const int pg = tok / kPage;
+    if (seen && pg < npages && ind_lo >= 0 && ind_lo + pg < p.num_indices)
+      page = p.kv_indices[ind_lo + pg];
+    if (page >= p.num_pages) page = -1;
+    // an absent page's rows are zeros
+    const int64_t blk = ((int64_t)max(page, 0) * 2 * p.hkv + h);
+    const uint8_t* k = p.cache + (blk * kPage + tok % kPage) * (int64_t)(D * ESZ);
+    float s = 0.f;
+    if (page >= 0)
+      for (int d = 0; d < D; ++d) s = __builtin_fmaf(h2f<BF16>(q[d]), value(k + d * ESZ), s);
+    s *= p.scale_log2;
+    float vs = 1.f;
+    if constexpr (FP8) {
+      if (page >= 0) {
+        s *= p.kv_scales[blk];
+        vs = p.kv_scales[blk + p.hkv];
+      }
+    }
+    if (!seen) s = -INFINITY;
+    float mx = s;
+#pragma unroll
+    for (int off = kWave / 2; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    const float m_new = fmaxf(m, mx);
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    const float w =
+        s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - (m == -INFINITY ? 0.f : m));
+    float sum = w;
+#pragma unroll
+    for (int off = kWave / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+    l = l * alpha + sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= alpha;
+    uint64_t rows = __builtin_amdgcn_ballot_w64(seen && page >= 0);
+    while (rows) {
+      const int i = __builtin_ctzll(rows);
+      rows &= rows - 1;
+      const float wi = lane_value(w, i) * lane_value(vs, i);
+      const int64_t b0 = (int64_t)__builtin_amdgcn_readlane(max(page, 0), i) * 2 * p.hkv + p.hkv + h;
+      const uint8_t* v = p.cache + (b0 * kPage + i % kPage) * (int64_t)(D * ESZ);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        o[e] = __builtin_fmaf(wi, value(v + (lane * E + e) * ESZ), o[e]);
+    }
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+template <int D, bool BF16, bool FP8, int RB, bool SPLIT, bool WINDOW>
 __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillParams p) {
   using C = PrefillCfg<D, BF16, FP8, RB>;
   constexpr int BN = C::BN;
@@ -332,7 +420,22 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       p.causal ? min(kv_len, max(0, diag + q_hi)) : kv_len;
   const int clean_end =
       p.causal ? min(kv_len, max(0, diag + q_lo + 1)) : kv_len;
-  const int n_tiles = (kv_end + BN - 1) / BN;
+  // a windowed tile walks the KV tiles that some row of it sees; tile t of the
+  // walk is KV tile kv_tile(t)
+  WindowTiles wt{0, 0, 0};
+  if constexpr (WINDOW)
+    wt = window_tiles(kv_end, (int64_t)diag + q_lo, p.window_left, p.sinks);
+  auto kv_tile = [&](int t) {
+    if constexpr (WINDOW) return t < wt.sink_tiles ? t : t - wt.sink_tiles + wt.first;
+    else return t;
+  };
+  // pages whose tokens no row of the tile sees are not read: [dead_lo, dead_hi)
+  int dead_lo = 0, dead_hi = 0;
+  if constexpr (WINDOW) {
+    dead_lo = (int)(((int64_t)p.sinks + kPage - 1) / kPage);
+    dead_hi = max(0, diag + q_lo - p.window_left) / kPage;
+  }
+  const int n_tiles = WINDOW ? wt.total : (kv_end + BN - 1) / BN;
   // the KV tiles [t_lo, t_hi) of this workgroup: all of them, or piece k of n
   int t_lo = 0, t_hi = n_tiles, slot = -1;
   if constexpr (SPLIT) {
@@ -364,6 +467,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
     // ---- Q^T fragments (B operand): lane -> row, 8 consecutive d per k-step
     u32x4 qf[RB][C::KS];
     int lim[RB];       // last visible kv index of the lane's row
+    int wlo[RB];       // WINDOW: first one past the sinks
     bool rvalid[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
@@ -371,6 +475,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       const int qi = q_lo + row / g;
       rvalid[rb] = qi < q_hi;
       lim[rb] = p.causal ? min(diag + qi, kv_len - 1) : kv_len - 1;
+      if constexpr (WINDOW) wlo[rb] = max(0, diag + qi - p.window_left);
       const uint16_t* qp =
           p.q + (int64_t)(qo_start + (rvalid[rb] ? qi : q_lo)) * p.q_sn +
           (int64_t)(h * g + row % g) * p.q_sh + 8 * half;
@@ -414,20 +519,23 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
                                   4 * dt + 2 * (qg & 1) + ((L & 3) >> 1)) +
                        8 * (L & 1);
 
+    auto fetch_ids = [&](int t) {
+      return fetch_seen_ids<WINDOW>(p, ind_lo, npages, kv_tile(t), lane, dead_lo, dead_hi);
+    };
     HalfRegs<D, BF16, FP8, RB> kr, vr;  // e4m3 staging only
     float ksc_l = 0.f, vsc_l = 0.f;     // e4m3 scales of the computed tile
-    int pid = fetch_page_ids(p, ind_lo, npages, t_lo, lane);
+    int pid = fetch_ids(t_lo);
     if (t_lo < t_hi) {
       if constexpr (FP8) {
-        load_half<D, BF16, FP8, RB, false>(kr, p, h, pid, npages, last, t_lo, wave, lane);
-        load_half<D, BF16, FP8, RB, true>(vr, p, h, pid, npages, last, t_lo, wave, lane);
+        load_half<D, BF16, FP8, RB, false>(kr, p, h, pid, npages, last, kv_tile(t_lo), wave, lane);
+        load_half<D, BF16, FP8, RB, true>(vr, p, h, pid, npages, last, kv_tile(t_lo), wave, lane);
       } else {
-        dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid, npages, last, t_lo, st0, wave, lane);
-        dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid, npages, last, t_lo, st0 + C::TILEB,
+        dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid, npages, last, kv_tile(t_lo), st0, wave, lane);
+        dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid, npages, last, kv_tile(t_lo), st0 + C::TILEB,
                                              wave, lane);
       }
     }
-    int pid_next = fetch_page_ids(p, ind_lo, npages, t_lo + 1, lane);
+    int pid_next = fetch_ids(t_lo + 1);
 
     // Tile t's QK, softmax and PV from stage `cur` (e4m3: with the register
     // loads of tile t + 1, pages pid_ld, issued between its phases).
@@ -448,13 +556,13 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
         }
         if (mt == 0) {
           if constexpr (FP8)
-            load_half<D, BF16, FP8, RB, false>(kr, p, h, pid_ld, npages, last, t + 1, wave, lane);
+            load_half<D, BF16, FP8, RB, false>(kr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
         }
       }
 
       // ---- online softmax in log2 units; lane holds 32 of the tile's 64
       // tokens of its row (token 32 mt + 8 (i/4) + 4 half + i%4 in register i)
-      const int tok0 = t * BN;
+      const int tok0 = kv_tile(t) * BN;
       float ksc[4], vsc[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -470,6 +578,17 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (32 * mt + 8 * (i >> 2) + (i & 3) > rel) s[rb][mt][i] = -INFINITY;
+          if constexpr (WINDOW) {
+            const int rel_lo = wlo[rb] - tok0 - 4 * half;  // and offset >= rel_lo, or a sink
+            const int rel_sink = p.sinks - tok0 - 4 * half;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int at = 32 * mt + 8 * (i >> 2) + (i & 3);
+                if (at < rel_lo && at >= rel_sink) s[rb][mt][i] = -INFINITY;
+              }
+          }
         }
         // e4m3: the page scale (> 0; FLT_MIN stands in for an empty page,
         // whose K rows are zero) multiplies each page's max once and enters
@@ -523,7 +642,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       for (int st = 0; st < 4; ++st) {
         if (st == 1) {
           if constexpr (FP8)
-            load_half<D, BF16, FP8, RB, true>(vr, p, h, pid_ld, npages, last, t + 1, wave, lane);
+            load_half<D, BF16, FP8, RB, true>(vr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
         }
         u32x4 pb[RB];
 #pragma unroll
@@ -570,13 +689,13 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
       pid = pid_next;
-      pid_next = fetch_page_ids(p, ind_lo, npages, t + 2, lane);
+      pid_next = fetch_ids(t + 2);
       const int pid_ld = t + 1 < t_hi ? pid : -1;  // past the last tile: no pages
       if constexpr (!FP8) {
         // tile t + 1 straight into the other stage, K and V, a whole tile
         // ahead of the barrier that waits for it
-        dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid_ld, npages, last, t + 1, nxt, wave, lane);
-        dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid_ld, npages, last, t + 1, nxt + C::TILEB,
+        dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1), nxt, wave, lane);
+        dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1), nxt + C::TILEB,
                                              wave, lane);
       }
       // paired tiles: a wave with no row of the tile only loads
@@ -587,7 +706,19 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
     // tiles [0, n_clean) lie wholly at or below the first row's diagonal
     // (and inside the sequence): no mask; the rest are masked.  Tile t uses
     // stage (t - t_lo) & 1 (the prologue loaded tile t_lo into stage 0).
-    const int n_clean = min(t_hi, SPLIT ? max(t_lo, clean_end / BN) : clean_end / BN);
+    // Windowed: the tiles before the last row's first token past the sinks are
+    // masked too, [t_lo, n_edge), unless no row's window leaves anything out.
+    int n_edge = t_lo, n_clean = 0;
+    if constexpr (WINDOW) {
+      const int last_lo = diag + q_hi - 1 - p.window_left;
+      if (last_lo > p.sinks)
+        n_edge = max(t_lo, min(t_hi, wt.sink_tiles + max(0, (last_lo + BN - 1) / BN - wt.first)));
+      n_clean = min(t_hi, max(n_edge, last_lo > p.sinks
+                                          ? wt.sink_tiles + max(0, clean_end / BN - wt.first)
+                                          : min(clean_end / BN, n_tiles)));
+    } else {
+      n_clean = min(t_hi, SPLIT ? max(t_lo, clean_end / BN) : clean_end / BN);
+    }
     int t = t_lo;
     auto run_tiles = [&](auto mask_tag, const int t_end) __attribute__((always_inline)) {
       if (t < t_end && ((t - t_lo) & 1)) {
@@ -617,19 +748,20 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), as in step
         __syncthreads();
         pid = pid_next;
-        pid_next = fetch_page_ids(p, ind_lo, npages, t + 2, lane);
+        pid_next = fetch_ids(t + 2);
         const int pid_ld = t + 1 < t_hi ? pid : -1;
         if constexpr (FP8) {
-          load_half<D, BF16, FP8, RB, false>(kr, p, h, pid_ld, npages, last, t + 1, wave, lane);
-          load_half<D, BF16, FP8, RB, true>(vr, p, h, pid_ld, npages, last, t + 1, wave, lane);
+          load_half<D, BF16, FP8, RB, false>(kr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
+          load_half<D, BF16, FP8, RB, true>(vr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
         } else {
-          dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid_ld, npages, last, t + 1, nxt, wave,
+          dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1), nxt, wave,
                                                 lane);
-          dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid_ld, npages, last, t + 1,
+          dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1),
                                                nxt + C::TILEB, wave, lane);
         }
       }
     }
+    if constexpr (WINDOW) run_tiles(std::true_type{}, n_edge);
     run_tiles(std::false_type{}, n_clean);
     run_tiles(std::true_type{}, t_hi);
     // the last tile's loads (of no page) are complete before the workgroup
@@ -640,7 +772,44 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const float2 lh = swap_halves32(l[rb]);
-      const float l_tot = lh.x + lh.y;
+      float l_tot = lh.x + lh.y;
+      if constexpr (WINDOW) {
+        // rows that are not finite, one by one (window_row)
+        float x = l_tot * 0.f;
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x = __builtin_fmaf(o[rb][dt][i], 0.f, x);
+        const float2 xh = swap_halves32(x);
+        uint32_t bad = (uint32_t)__builtin_amdgcn_ballot_w64(rvalid[rb] && !(xh.x + xh.y == 0.f));
+        while (bad) {
+          const int i = __builtin_ctz(bad);
+          bad &= bad - 1;
+          const int row = 32 * (RB * wave + rb) + i;
+          const int qi = q_lo + row / g;
+          const int head = h * g + row % g;
+          float ro[D / kWave], rm, rl;
+          window_row<D, BF16, FP8>(
+              p, h, ind_lo, npages, kv_len, diag + qi, __builtin_amdgcn_readlane(lim[rb], i), wt,
+              t_lo, t_hi, p.q + (int64_t)(qo_start + qi) * p.q_sn + (int64_t)head * p.q_sh, lane,
+              ro, &rm, &rl);
+          // into the accumulators of the row's lanes i and i + 32: element
+          // 32 dt + 8 i4 + 4 half + k of the row is register 4 i4 + k of tile dt
+#pragma unroll
+          for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int d = 32 * dt + 8 * (r >> 2) + (r & 3);
+              const float lo = lane_value(ro[d % (D / kWave)], d / (D / kWave));
+              const float hi = lane_value(ro[(d + 4) % (D / kWave)], (d + 4) / (D / kWave));
+              if (col == i) o[rb][dt][r] = half ? hi : lo;
+            }
+          if (col == i) {
+            m[rb] = rm;
+            l_tot = rl;
+          }
+        }
+      }
       if constexpr (SPLIT) {
         if (slot >= 0) {
           if (!wave_rows) continue;
@@ -841,18 +1010,26 @@ __global__ void __launch_bounds__(kWave * kPrefillMergeWaves)
 using PrefillFn = void (*)(PrefillParams);
 
 template <int D, bool BF16, bool FP8>
-PrefillFn prefill_fn(bool split) {
-  return split ? prefill_kernel<D, BF16, FP8, kPrefillRB, true>
-               : prefill_kernel<D, BF16, FP8, kPrefillRB, false>;
+PrefillFn prefill_fn(bool split, bool window) {
+  if (window)
+    return split ? prefill_kernel<D, BF16, FP8, kPrefillRB, true, true>
+                 : prefill_kernel<D, BF16, FP8, kPrefillRB, false, true>;
+  return split ? prefill_kernel<D, BF16, FP8, kPrefillRB, true, false>
+               : prefill_kernel<D, BF16, FP8, kPrefillRB, false, false>;
 }
 
-static PrefillFn pick_prefill(int d, bool bf16, bool fp8, bool split) {
-  if (d == 64) {
-    if (bf16) return fp8 ? prefill_fn<64, true, true>(split) : prefill_fn<64, true, false>(split);
-    return fp8 ? prefill_fn<64, false, true>(split) : prefill_fn<64, false, false>(split);
-  }
-  if (bf16) return fp8 ? prefill_fn<128, true, true>(split) : prefill_fn<128, true, false>(split);
-  return fp8 ? prefill_fn<128, false, true>(split) : prefill_fn<128, false, false>(split);
+template <int D>
+PrefillFn prefill_fn_d(bool bf16, bool fp8, bool split, bool window) {
+  if (bf16)
+    return fp8 ? prefill_fn<D, true, true>(split, window)
+               : prefill_fn<D, true, false>(split, window);
+  return fp8 ? prefill_fn<D, false, true>(split, window)
+             : prefill_fn<D, false, false>(split, window);
+}
+
+static PrefillFn pick_prefill(int d, bool bf16, bool fp8, bool split, bool window) {
+  return d == 64 ? prefill_fn_d<64>(bf16, fp8, split, window)
+                 : prefill_fn_d<128>(bf16, fp8, split, window);
 }
 
 // ----------------------------------------------------------------------------
@@ -882,6 +1059,7 @@ struct PrefillPlanArgs {
   PrefillPiece* pieces;
   PrefillMerge* merges;
   int32_t* n_merge;
+  int32_t window_left, sinks;
 };
 
 constexpr int kPrefillPlanThreads = 1024;
@@ -946,6 +1124,9 @@ __global__ void __launch_bounds__(kPrefillPlanThreads) prefill_plan_kernel(Prefi
       const int last = min(max(a.last_page_len[b], 1), kPage);
       const int64_t kv_len = np > 0 ? (int64_t)(np - 1) * kPage + last : 0;
       *cost = max<int64_t>(0, min<int64_t>(kv_len, kv_len - qo + q_hi));
+      if (a.window_left >= 0)
+        *cost = (int64_t)kPrefillKvTile *
+                window_tiles(*cost, kv_len - qo + q_lo, a.window_left, a.sinks).total;
     }
     const int flag = a.pair && (int64_t)(q_hi - q_lo) * a.g <= kPrefillRows / 2 ? 1 : -1;
     return PrefillItem{b, q_lo, q_hi, flag};
@@ -1067,7 +1248,8 @@ static int launch_prefill_plan(const pagedattn_plan* plan, const int32_t* qo_ind
                     reinterpret_cast<int32_t*>(static_cast<char*>(plan->workspace) + 12),
                     plan->scratch_bytes ? plan->n_slots : 0, plan->n_pieces,
                     static_cast<PrefillPiece*>(plan->pieces_dev),
-                    static_cast<PrefillMerge*>(plan->merge_dev), plan->n_merge_dev};
+                    static_cast<PrefillMerge*>(plan->merge_dev), plan->n_merge_dev,
+                    plan->window_left, plan->sinks};
   hipLaunchKernelGGL(prefill_plan_kernel, dim3(1), dim3(kPrefillPlanThreads), 0,
                      (hipStream_t)stream, a);
   return check_launch(who);
@@ -1188,13 +1370,15 @@ int pagedattn_prefill_run_scratch(const pagedattn_plan* plan, const void* q,
   p.hkv = plan->hkv;
   p.g = plan->hq / plan->hkv;
   p.causal = causal ? 1 : 0;
+  p.window_left = plan->window_left;
+  p.sinks = plan->sinks;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.partial_o = cut ? static_cast<float*>(scratch) : nullptr;
   p.partial_lse =
       cut ? reinterpret_cast<float*>(static_cast<char*>(scratch) + plan->scratch_lse) : nullptr;
   p.n_slots = cut ? plan->n_slots : 0;
   const bool bf16 = q_dtype == PAGEDATTN_BF16;
-  PrefillFn fn = pick_prefill(plan->d, bf16, fp8, cut);
+  PrefillFn fn = pick_prefill(plan->d, bf16, fp8, cut, plan->window_left >= 0);
   if (plan->implicit && !plan->dev_table) {
     // the work list of this run, built on the device ahead of the attention
     // (unless pagedattn_prefill_plan_device_update built it for the step)

@@ -102,9 +102,23 @@ int pagedattn_prefill_plan(pagedattn_plan* plan, const int32_t* qo_indptr_host,
                            int32_t num_kv_heads, int32_t head_dim,
                            int32_t page_size, void* workspace,
                            size_t workspace_bytes, void* stream) {
+  return pagedattn_prefill_plan_window(plan, qo_indptr_host, kv_indptr_host,
+                                       kv_last_page_len_host, batch_size, num_qo_heads,
+                                       num_kv_heads, head_dim, page_size, -1, 0, workspace,
+                                       workspace_bytes, stream);
+}
+
+int pagedattn_prefill_plan_window(pagedattn_plan* plan, const int32_t* qo_indptr_host,
+                                  const int32_t* kv_indptr_host,
+                                  const int32_t* kv_last_page_len_host,
+                                  int32_t batch_size, int32_t num_qo_heads,
+                                  int32_t num_kv_heads, int32_t head_dim,
+                                  int32_t page_size, int32_t window_left, int32_t sinks,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "prefill_plan";
   if (!plan) return set_error(PAGEDATTN_ERR_INVALID, "%s: null plan", who);
   plan->mode = kPlanNone;
+  if (check_window(who, window_left, sinks)) return PAGEDATTN_ERR_INVALID;
   plan->scratch_bytes = 0;
   if (batch_size < 0)
     return set_error(PAGEDATTN_ERR_INVALID, "%s: batch_size %d < 0", who,
@@ -148,6 +162,8 @@ int pagedattn_prefill_plan(pagedattn_plan* plan, const int32_t* qo_indptr_host,
     pl->d = head_dim;
     pl->page_size = page_size;
     pl->q_tile = q_tile;
+    pl->window_left = window_left;
+    pl->sinks = sinks;
     pl->total_qo =
         batch_size > 0 ? (int64_t)qo_indptr_host[batch_size] - qo_indptr_host[0] : 0;
     pl->implicit = false;
@@ -167,9 +183,15 @@ int pagedattn_prefill_plan(pagedattn_plan* plan, const int32_t* qo_indptr_host,
       // D = 64 -- run it like any other)
       const int flag = pair && (int64_t)(hi - lo) * g <= kPrefillRows / 2 ? 1 : -1;
       items.push_back(PrefillItem{b, lo, hi, flag});
-      // kv tokens the tile's last row can see (causal)
-      cost.push_back(std::max<int64_t>(
-          0, std::min<int64_t>(kv_len[b], (int64_t)kv_len[b] - qo + hi)));
+      // kv tokens the tile's last row can see (causal); with a window, those
+      // of the KV tiles that the tile reads
+      const int64_t end = std::max<int64_t>(
+          0, std::min<int64_t>(kv_len[b], (int64_t)kv_len[b] - qo + hi));
+      cost.push_back(window_left < 0
+                         ? end
+                         : (int64_t)kPrefillKvTile *
+                               window_tiles(end, (int64_t)kv_len[b] - qo + lo, window_left, sinks)
+                                   .total);
     }
   }
   // most expensive tiles first
@@ -237,9 +259,21 @@ int pagedattn_prefill_plan_device(pagedattn_plan* plan, int32_t batch_size,
                                   int32_t num_qo_heads, int32_t num_kv_heads,
                                   int32_t head_dim, int32_t page_size, int64_t max_qo_tokens,
                                   void* workspace, size_t workspace_bytes) {
+  return pagedattn_prefill_plan_device_window(plan, batch_size, num_qo_heads, num_kv_heads,
+                                              head_dim, page_size, max_qo_tokens, -1, 0,
+                                              workspace, workspace_bytes);
+}
+
+int pagedattn_prefill_plan_device_window(pagedattn_plan* plan, int32_t batch_size,
+                                         int32_t num_qo_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, int32_t page_size,
+                                         int64_t max_qo_tokens, int32_t window_left,
+                                         int32_t sinks, void* workspace,
+                                         size_t workspace_bytes) {
   const char* who = "prefill_plan_device";
   if (!plan) return set_error(PAGEDATTN_ERR_INVALID, "%s: null plan", who);
   plan->mode = kPlanNone;
+  if (check_window(who, window_left, sinks)) return PAGEDATTN_ERR_INVALID;
   plan->scratch_bytes = 0;
   if (batch_size < 0 || batch_size > kPrefillDevMaxBatch)
     return set_error(PAGEDATTN_ERR_UNSUPPORTED, "%s: batch_size %d outside [0, %d]", who,
@@ -277,6 +311,8 @@ int pagedattn_prefill_plan_device(pagedattn_plan* plan, int32_t batch_size,
   plan->n_merge = 0;
   plan->n_slots = 0;
   plan->q_tile = q_tile;
+  plan->window_left = window_left;
+  plan->sinks = sinks;
   plan->total_qo = max_qo_tokens;
   plan->items_dev = static_cast<char*>(workspace) + kWsHeader;
   // the plan kernel may cut tiles, on the host plan's rule (the tiles are known

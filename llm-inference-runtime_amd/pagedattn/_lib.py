@@ -98,6 +98,25 @@ _SIGNATURES = {
         [_c_p, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
          _c_int, _c_p, _c_f, _c_f, _c_p, _c_int, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_p,
          _c_p, _c_f, _c_p, _c_sz, _c_p]),
+    "pagedattn_decode_window_metadata": (
+        _c_int,
+        [_c_p, _c_p, _c_int, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p, _c_int, _c_p, _c_p]),
+    "pagedattn_decode_plan_window": (
+        _c_int,
+        [_c_p, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_p, _c_sz, _c_p]),
+    "pagedattn_decode_run_window": (
+        _c_int,
+        [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_int, _c_p, _c_f, _c_f, _c_p, _c_int, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_p,
+         _c_p, _c_f, _c_p, _c_sz, _c_p]),
+    "pagedattn_prefill_plan_window": (
+        _c_int,
+        [_c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_p, _c_sz, _c_p]),
+    "pagedattn_prefill_plan_device_window": (
+        _c_int, [_c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_p,
+                 _c_sz]),
     "pagedattn_decode_plan_device": (
         _c_int, [_c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_sz]),
     "pagedattn_decode_plan_device_update": (_c_int, [_c_p, _c_p, _c_p, _c_p]),

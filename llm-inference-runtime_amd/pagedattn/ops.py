@@ -14,8 +14,10 @@ meaning and error behaviour (Python exceptions, never a device fault):
 
 Only the "HND" pool layout the engine uses is implemented
 ([num_pages, 2, num_kv_heads, page_size, head_dim] per layer).  Options the
-engine never passes (positional encoding inside attention, sliding windows,
-logit soft-capping, custom masks) raise NotImplementedError.
+engine never passes (positional encoding inside attention, logit soft-capping,
+custom masks) raise NotImplementedError.  Both wrappers take FlashInfer's
+``window_left`` (sliding window) at ``plan``, and with it ``num_sink_tokens``
+(first tokens that stay visible, which FlashInfer has no argument for).
 
 Additions with no FlashInfer counterpart: ``build_paged_metadata`` (the
 step metadata built on the device), ``quantize_pages_e4m3``, the
@@ -27,6 +29,7 @@ scales as pages fill) and ``fork_pages`` (copy-on-write page fork).
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -547,22 +550,40 @@ class _Plan:
             self.handle = None
 
 
-def _unsupported_options(pos_encoding_mode="NONE", window_left=-1, logits_soft_cap=None,
+def _unsupported_options(pos_encoding_mode="NONE", logits_soft_cap=None,
                          custom_mask=None, packed_custom_mask=None) -> None:
     if pos_encoding_mode not in ("NONE", None):
         raise NotImplementedError(
             f"pos_encoding_mode={pos_encoding_mode!r}: RoPE is applied by "
             "apply_rope_pos_ids_inplace before attention")
-    if window_left not in (-1, None):
-        raise NotImplementedError("sliding-window attention is not implemented")
     if logits_soft_cap not in (None, 0, 0.0):
         raise NotImplementedError("logits_soft_cap is not implemented")
     if custom_mask is not None or packed_custom_mask is not None:
         raise NotImplementedError("custom masks are not implemented")
 
 
+def _window(window_left, num_sink_tokens) -> tuple[int, int]:
+    """(window_left, sinks) of a plan; (-1, 0) without a window."""
+    left = -1 if window_left is None else operator.index(window_left)
+    sinks = operator.index(num_sink_tokens)
+    if left < -1 or left >= 1 << 31:
+        raise ValueError(f"window_left {left}: the tokens seen before a token, or -1 for all")
+    if sinks < 0 or sinks >= 1 << 31:
+        raise ValueError(f"num_sink_tokens {sinks} is negative or too large")
+    if left < 0 and sinks > 0:
+        raise ValueError("num_sink_tokens needs a window (window_left >= 0)")
+    return left, sinks
+
+
 class _WrapperBase:
     _graph_capable = False
+    _window_left = -1
+
+    def _check_window(self, window_left) -> None:
+        """forward()'s window: the planned one (-1 and None stand for it)."""
+        if window_left not in (-1, None) and window_left != self._window_left:
+            raise ValueError(f"forward with window_left {window_left}, the plan has "
+                             f"{self._window_left}: the window is given to plan()")
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
                  use_cuda_graph: bool = False, **_unused):
@@ -641,17 +662,24 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
              rope_scale=None, rope_theta=None, non_blocking: bool = True,
              split_pages: int = 0, device_plan: bool = False,
              indptr_host: torch.Tensor | None = None,
-             last_page_len_host: torch.Tensor | None = None, **_unused) -> None:
+             last_page_len_host: torch.Tensor | None = None, num_sink_tokens: int = 0,
+             **_unused) -> None:
         """indptr_host / last_page_len_host: CPU copies of indptr and
         last_page_len that the caller already holds; the plan then makes no
-        device-to-host copy of its own."""
-        _unsupported_options(pos_encoding_mode, window_left, logits_soft_cap)
+        device-to-host copy of its own.
+
+        window_left = w >= 0: every sequence's query, its newest token, sees the
+        w tokens before it and itself, and the first num_sink_tokens tokens.
+        Pages it does not see are not read (their entries may be -1)."""
+        _unsupported_options(pos_encoding_mode, logits_soft_cap)
+        window = _window(window_left, num_sink_tokens)
         if page_size != PAGE_SIZE:
             raise NotImplementedError(f"page_size {page_size} (only 16 is implemented)")
         if self._use_graph or device_plan:
             self._plan_device(indptr, indices, last_page_len, num_qo_heads, num_kv_heads,
                               head_dim, page_size, q_data_type, kv_data_type, data_type,
                               sm_scale)
+            self._set_window(window, lists_now=False)
             return
         device = self._ws.device
         indptr_h = _host_i32(indptr if indptr_host is None else indptr_host)
@@ -668,15 +696,41 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
             raise ValueError(f"indices has {indices.numel()} entries, indptr needs {n_ind}")
         self._q_dtype = _dtype_of(data_type if data_type is not None else q_data_type)
         self._kv_dtype = _dtype_of(kv_data_type) if kv_data_type is not None else None
-        call("pagedattn_decode_plan", self._plan.handle, ptr(indptr_h), ptr(last_h), bsz,
+        call("pagedattn_decode_plan_window", self._plan.handle, ptr(indptr_h), ptr(last_h), bsz,
              int(num_qo_heads), int(num_kv_heads), int(head_dim), int(page_size),
-             int(split_pages), ptr(self._ws), self._ws_bytes, _stream(device))
+             int(split_pages), *window, ptr(self._ws), self._ws_bytes, _stream(device))
         self._indptr = _i32(indptr, device)
         self._indices = _i32(indices, device)
         self._last = _i32(last_page_len, device)
         self._bsz, self._hq, self._hkv, self._d = bsz, int(num_qo_heads), int(num_kv_heads), int(head_dim)
         self._sm_scale = sm_scale
         self._planned = True
+        self._set_window(window, lists_now=True)
+
+    def _set_window(self, window: tuple[int, int], lists_now: bool) -> None:
+        """The buffers of the lists of visible pages that a windowed plan's runs
+        read, filled now (a host plan) or ahead of the runs (a device plan)."""
+        self._window_left, self._sinks = left, sinks = window
+        self._holes = None
+        self._lists_made = lists_now
+        if left < 0:
+            return
+        self._planned = False
+        n, device = self._bsz, self._indptr.device
+        per_seq = -(-sinks // PAGE_SIZE) + left // PAGE_SIZE + 2
+        room = min(self._indices.numel(), n * per_seq)
+        self._seen_indptr = torch.zeros(n + 1, dtype=torch.int32, device=device)
+        self._seen_indices = torch.empty(max(room, 1), dtype=torch.int32, device=device)[:room]
+        self._holes = torch.empty((max(n, 1), 4), dtype=torch.int32, device=device)[:n]
+        if lists_now:
+            self._make_lists()
+        self._planned = True
+
+    def _make_lists(self) -> None:
+        call("pagedattn_decode_window_metadata", ptr(self._indptr), ptr(self._indices),
+             self._indices.numel(), ptr(self._last), self._bsz, self._window_left, self._sinks,
+             ptr(self._seen_indptr), ptr(self._seen_indices), self._seen_indices.numel(),
+             ptr(self._holes), _stream(self._indptr.device))
 
     def _plan_device(self, indptr, indices, last_page_len, num_qo_heads, num_kv_heads,
                      head_dim, page_size, q_data_type, kv_data_type, data_type, sm_scale):
@@ -718,14 +772,22 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         Until the next plan(), every run reads that deal instead of making
         its own in its prologue, so the metadata must not change between
         this call and the runs it serves: an engine step calls it once after
-        writing the step's metadata, before the layers' runs.  A no-op for
-        host plans and for device plans of the split kind."""
+        writing the step's metadata, before the layers' runs.  A windowed
+        device plan's lists of visible pages are made here too (without this
+        call, ahead of every run).  A no-op for host plans and, without a
+        window, for device plans of the split kind."""
         if not self._planned:
             raise RuntimeError("plan() must be called before update_plan()")
-        if self.plan_kind != "device_shared":
+        kind = self.plan_kind
+        if kind not in ("device", "device_shared"):
             return
-        call("pagedattn_decode_plan_device_update", self._plan.handle, ptr(self._indptr),
-             ptr(self._last), _stream(self._indptr.device))
+        if self._holes is not None:
+            self._make_lists()
+            self._lists_made = True
+        if kind == "device_shared":
+            call("pagedattn_decode_plan_device_update", self._plan.handle,
+                 ptr(self._indptr if self._holes is None else self._seen_indptr),
+                 ptr(self._last), _stream(self._indptr.device))
 
     @property
     def plan_kind(self) -> str | None:
@@ -760,9 +822,14 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         entry = ("pagedattn_decode_run" if append_key is None else
                  "pagedattn_decode_run_append" if rope is None else
                  "pagedattn_decode_run_rope_append")
-        r = _native("decode_run", entry, self._plan.handle, q, paged_kv_cache, self._indices,
-                    self._indptr, self._last, self._bsz, self._hq, self._hkv, self._d, kv_scales,
-                    out, lse, return_lse, scale, append_key, append_value, rope, positions)
+        indices, indptr, holes = self._indices, self._indptr, self._holes
+        if holes is not None:
+            if not self._lists_made:
+                self._make_lists()
+            indices, indptr = self._seen_indices, self._seen_indptr
+        r = _native("decode_run", entry, self._plan.handle, q, paged_kv_cache, indices, indptr,
+                    self._last, self._bsz, self._hq, self._hkv, self._d, kv_scales, out, lse,
+                    return_lse, scale, append_key, append_value, rope, positions, holes)
         if r is not NotImplemented:
             return r
         num_pages, _, _ = _check_pool(paged_kv_cache, self._hkv, self._d, self._kv_layout)
@@ -778,7 +845,7 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         if return_lse and lse is None:
             lse = torch.empty((self._bsz, self._hq), dtype=torch.float32, device=q.device)
         common = (ptr(paged_kv_cache), dtype_code(paged_kv_cache.dtype), ptr(scales),
-                  num_pages, ptr(self._indices), self._indices.numel(), ptr(self._indptr),
+                  num_pages, ptr(indices), indices.numel(), ptr(indptr),
                   ptr(self._last), ptr(out), ptr(lse), float(scale))
         if append_key is None and append_value is None:
             rows = (None, None, 0, 0, 0, 0, 0, None, 1.0, 1.0)
@@ -804,9 +871,9 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
             rows = (ptr(append_key), ptr(append_value), append_key.stride(0),
                     append_key.stride(1), append_value.stride(0), append_value.stride(1),
                     *rotate)
-        _run_plan(entry, "pagedattn_decode_run_scratch", _scratch(self._plan, q), q.device,
-                  self._plan.handle, ptr(q), q.stride(0), q.stride(1), dtype_code(q.dtype), *rows,
-                  *common)
+        _run_plan(entry, "pagedattn_decode_run_window", _scratch(self._plan, q), q.device,
+                  self._plan.handle, ptr(holes), ptr(q), q.stride(0), q.stride(1),
+                  dtype_code(q.dtype), *rows, *common)
         return (out, lse) if return_lse else out
 
     def forward(self, q: torch.Tensor, paged_kv_cache: torch.Tensor,
@@ -814,7 +881,8 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
                 window_left: int = -1, logits_soft_cap: float | None = None,
                 sm_scale: float | None = None, rope_scale=None, rope_theta=None,
                 return_lse: bool = False, kv_scales: torch.Tensor | None = None):
-        _unsupported_options(pos_encoding_mode, window_left, logits_soft_cap)
+        _unsupported_options(pos_encoding_mode, logits_soft_cap)
+        self._check_window(window_left)
         if q_scale is not None or k_scale is not None or v_scale is not None:
             raise NotImplementedError("scalar q/k/v scales; pass per-page kv_scales")
         return self.run(q, paged_kv_cache, kv_scales=kv_scales, return_lse=return_lse,
@@ -843,9 +911,13 @@ class BatchPrefillWithPagedKVCacheWrapper(_WrapperBase):
              q_data_type="float16", kv_data_type=None, sm_scale: float | None = None,
              rope_scale=None, rope_theta=None, non_blocking: bool = True,
              device_plan: bool = False, max_qo_tokens: int | None = None,
-             **_unused) -> None:
-        _unsupported_options(pos_encoding_mode, window_left, logits_soft_cap, custom_mask,
+             num_sink_tokens: int = 0, **_unused) -> None:
+        """window_left = w >= 0: a row at position p sees positions j with
+        j >= p - w or j < num_sink_tokens (and j <= p if causal).  Pages that no
+        row of a sequence sees are not read (their entries may be -1)."""
+        _unsupported_options(pos_encoding_mode, logits_soft_cap, custom_mask,
                              packed_custom_mask)
+        window = _window(window_left, num_sink_tokens)
         if head_dim_vo is not None and head_dim_vo != head_dim_qk:
             raise NotImplementedError("head_dim_vo != head_dim_qk")
         if page_size != PAGE_SIZE:
@@ -865,15 +937,17 @@ class BatchPrefillWithPagedKVCacheWrapper(_WrapperBase):
             if qo_indptr.numel() != bsz + 1 or paged_kv_indptr.numel() != bsz + 1:
                 raise ValueError("qo_indptr and paged_kv_indptr need batch_size + 1 entries")
             self._q_dtype = _dtype_of(q_data_type)
-            call("pagedattn_prefill_plan_device", self._plan.handle, bsz, int(num_qo_heads),
-                 int(num_kv_heads), int(head_dim_qk), int(page_size), int(max_qo_tokens),
-                 ptr(self._ws), self._ws_bytes)
+            call("pagedattn_prefill_plan_device_window", self._plan.handle, bsz,
+                 int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size),
+                 int(max_qo_tokens), *window, ptr(self._ws), self._ws_bytes)
             self._qo_rows = None  # known on the device only
             self._device_plan = True
         else:
             self._plan_host(qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len,
-                            num_qo_heads, num_kv_heads, head_dim_qk, page_size, q_data_type)
+                            num_qo_heads, num_kv_heads, head_dim_qk, page_size, q_data_type,
+                            window)
             self._device_plan = False
+        self._window_left = window[0]
         self._qo_indptr = _i32(qo_indptr, device)
         self._indptr = _i32(paged_kv_indptr, device)
         self._indices = _i32(paged_kv_indices, device)
@@ -885,7 +959,8 @@ class BatchPrefillWithPagedKVCacheWrapper(_WrapperBase):
         self._planned = True
 
     def _plan_host(self, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len,
-                   num_qo_heads, num_kv_heads, head_dim_qk, page_size, q_data_type) -> None:
+                   num_qo_heads, num_kv_heads, head_dim_qk, page_size, q_data_type,
+                   window) -> None:
         device = self._ws.device
         qo_h = _host_i32(qo_indptr)
         indptr_h = _host_i32(paged_kv_indptr)
@@ -898,9 +973,9 @@ class BatchPrefillWithPagedKVCacheWrapper(_WrapperBase):
             raise ValueError(
                 f"paged_kv_indices has {paged_kv_indices.numel()} entries, indptr needs {n_ind}")
         self._q_dtype = _dtype_of(q_data_type)
-        call("pagedattn_prefill_plan", self._plan.handle, ptr(qo_h), ptr(indptr_h),
+        call("pagedattn_prefill_plan_window", self._plan.handle, ptr(qo_h), ptr(indptr_h),
              ptr(last_h), bsz, int(num_qo_heads), int(num_kv_heads), int(head_dim_qk),
-             int(page_size), ptr(self._ws), self._ws_bytes, _stream(device))
+             int(page_size), *window, ptr(self._ws), self._ws_bytes, _stream(device))
         self._qo_rows = int(qo_h[-1]) if bsz else 0
 
     begin_forward = plan
@@ -972,6 +1047,7 @@ class BatchPrefillWithPagedKVCacheWrapper(_WrapperBase):
                 logits_soft_cap: float | None = None, sm_scale: float | None = None,
                 rope_scale=None, rope_theta=None, return_lse: bool = False,
                 kv_scales: torch.Tensor | None = None, **_unused):
-        _unsupported_options(pos_encoding_mode, window_left, logits_soft_cap)
+        _unsupported_options(pos_encoding_mode, logits_soft_cap)
+        self._check_window(window_left)
         return self.run(q, paged_kv_cache, kv_scales=kv_scales, return_lse=return_lse,
                         causal=causal, sm_scale=sm_scale)

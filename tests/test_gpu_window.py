@@ -1,0 +1,359 @@
+"""Sliding-window attention with sinks, decode and prefill, against a plain
+implementation in 64 bits that only ever touches the tokens a row sees.
+
+The bound of an output element: the weights and the output are each rounded once
+to the 16-bit type (half a step u, relative), scores are sums of D products in
+32 bits, and a score that is off by s changes every weight by at most
+exp(2 s) - 1; fp16 weights below 2^-24 of a row's largest round to multiples
+of 2^-24."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import pagedattn
+from pagedattn.metadata import decode_metadata, prefill_metadata
+
+from paged_cases import i32, random_tables, require_shared_plans, strided_rows, workspace
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(32, 4, 64), (32, 8, 128), (8, 8, 64), (16, 1, 128)]
+
+
+def make(device, computed, chunks, heads, dtype, fp8, window, sinks, seed, spoil=True):
+    """A paged batch whose unseen tokens hold NaN and infinities (spoil) and whose
+    unseen pages are gone (-1) or name a page of NaN."""
+    hq, hkv, d = heads
+    rng = np.random.default_rng(seed)
+    lens = [c + n for c, n in zip(computed, chunks)]
+    tables, num_pages = random_tables(rng, lens, extra_pages=4)
+    meta = prefill_metadata(tables, computed, chunks)
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    pool = torch.randn((num_pages, 2, hkv, 16, d), generator=g, device=device)
+    scales = None
+    if fp8:
+        scales = (torch.rand((num_pages, 2, hkv), generator=g, device=device) + 0.5) / 64
+        pool = (pool / scales[..., None, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    else:
+        pool = pool.to(dtype)
+    q = strided_rows(meta.nnz, hq, d, dtype, device, g, tail=2 * hkv)
+    if spoil:
+        trash = sorted(set(range(num_pages)) - {p for t in tables for p in t})[0]
+        bad = [math.nan, math.nan] if fp8 else [math.nan, math.inf]
+        pool[trash] = math.nan
+        for b, (n, table) in enumerate(zip(lens, tables)):
+            first = n - chunks[b] - window  # the first token past the sinks that a row sees
+            for t in range(min(sinks, n), min(first, n)):
+                pool[table[t // 16], 0, :, t % 16] = bad[t % 2]
+                pool[table[t // 16], 1, :, t % 16] = bad[(t + 1) % 2]
+            lo, hi = -(-sinks // 16), max(first, 0) // 16
+            for s in range(lo, min(hi, len(table))):
+                meta.kv_indices[meta.kv_indptr[b] + s] = -1 if s % 2 else trash
+    return meta, pool, scales, q
+
+
+def rows64(pool, scales, ids, kind, tokens):
+    page = torch.as_tensor(ids, device=pool.device)[tokens // 16].long()
+    x = pool[page, kind, :, tokens % 16].double()
+    return x if scales is None else x * scales[page, kind].double()[..., None]
+
+
+def reference(meta, pool, scales, q, window, sinks, causal=True, b_rows=None, q_err=0.0):
+    """(out, lse, bound of out, bound of lse) in 64 bits; q_err: relative rounding of q."""
+    dev, (n, hq, d) = q.device, q.shape
+    hkv = pool.shape[2]
+    g = hq // hkv
+    u = torch.finfo(q.dtype).eps / 2
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    out = torch.zeros((n, hq, d), dtype=torch.float64, device=dev)
+    lse = torch.full((n, hq), -math.inf, dtype=torch.float64, device=dev)
+    out_tol, lse_tol = torch.zeros_like(out), torch.zeros_like(lse)
+    for b in range(len(meta.kv_last_page_len)):
+        ids = meta.kv_indices[meta.kv_indptr[b]:meta.kv_indptr[b + 1]]
+        length = (len(ids) - 1) * 16 + int(meta.kv_last_page_len[b]) if len(ids) else 0
+        r0, r1 = int(meta.qo_indptr[b]), int(meta.qo_indptr[b + 1])
+        for r in range(r0, r1):
+            if b_rows is not None and r not in b_rows:
+                continue
+            at = length - (r1 - r0) + r - r0
+            end = min(at + 1, length) if causal else length
+            tok = torch.arange(max(end, 0), device=dev)
+            tok = tok[(tok >= at - window) | (tok < sinks)]
+            if not tok.numel():
+                continue
+            k, v = (rows64(pool, scales, ids, i, tok).repeat_interleave(g, 1) for i in (0, 1))
+            x = q[r].double()[:, None]
+            s = (k.transpose(0, 1) * x).sum(-1) / math.sqrt(d)  # [hq, tokens]
+            size = (k.transpose(0, 1) * x).abs().sum(-1).amax(-1) / math.sqrt(d)
+            lse[r] = torch.logsumexp(s, -1)
+            p = torch.exp(s - lse[r][:, None])[..., None]
+            vt = v.transpose(0, 1)
+            out[r] = (p * vt).sum(1)
+            spread = (p * vt.abs()).sum(1)
+            off = size * (q_err + (d + 8) * 2.0 ** -24) + s.abs().amax(-1) * 2.0 ** -21
+            codes = vt.abs().amax(1) if scales is None else vt.abs().amax(1) * 64 * 2
+            out_tol[r] = (u * out[r].abs() + spread * (u * 1.01 + torch.expm1(2 * off)[:, None])
+                          + tok.numel() * tiny * codes
+                          * torch.exp(s.amax(-1) - lse[r])[:, None] + 2.0 ** -24)
+            lse_tol[r] = off + lse[r].abs() * 2.0 ** -21 + 2.0 ** -20
+    return out, lse, out_tol, lse_tol
+
+
+def check(out, lse, ref, rows=None):
+    want, want_lse, tol, lse_tol = ref
+    pick = slice(None) if rows is None else rows
+    got = out.double()[pick]
+    assert bool(torch.isfinite(got).all()), "an unseen token reached the output"
+    worst = ((got - want[pick]).abs() / tol[pick].clamp_min(1e-30)).max()
+    assert float(worst) <= 1, f"{float(worst)} times the bound"
+    if lse is not None:
+        a, b = lse.double()[pick], want_lse[pick]
+        assert torch.equal(torch.isinf(a), torch.isinf(b))
+        live = ~torch.isinf(b)
+        assert bool(((a - b).abs()[live] <= lse_tol[pick][live]).all())
+
+
+def plan_decode(device, meta, heads, dtype, window, sinks, kind, ws=None):
+    w = pagedattn.BatchDecodeWithPagedKVCacheWrapper(
+        workspace(device) if ws is None else ws, "HND")
+    w.plan(i32(meta.kv_indptr, device), i32(meta.kv_indices, device),
+           i32(meta.kv_last_page_len, device), *heads, 16, q_data_type=dtype, window_left=window,
+           num_sink_tokens=sinks, device_plan=kind == "device",
+           split_pages={"split": 4, "whole": -1}.get(kind, 0))
+    return w
+
+
+LENS = [1, 16, 17, 40, 129, 130, 145, 300, 1000]
+
+
+@pytest.mark.parametrize("kind", ["host", "split", "whole", "device"])
+@pytest.mark.parametrize("window,sinks", [(127, 4), (0, 0), (16, 16), (30, 1), (200, 33),
+                                          (5, 40), (100000, 3)])
+@pytest.mark.parametrize("heads,dtype,fp8", [
+    (HEADS[0], torch.float16, False), (HEADS[1], torch.bfloat16, False),
+    (HEADS[1], torch.bfloat16, True), (HEADS[2], torch.float16, True),
+    (HEADS[3], torch.bfloat16, False)])
+def test_decode(gpu, heads, dtype, fp8, window, sinks, kind):
+    meta, pool, scales, q = make(gpu, [n - 1 for n in LENS], [1] * len(LENS), heads, dtype, fp8,
+                                 window, sinks, seed=window + sinks)
+    w = plan_decode(gpu, meta, heads, dtype, window, sinks, kind)
+    out, lse = w.run(q, pool, kv_scales=scales, return_lse=True)
+    check(out, lse, reference(meta, pool, scales, q, window, sinks))
+
+
+@pytest.mark.parametrize("kind", ["host", "device"])
+def test_decode_many_sequences(gpu, kind):
+    """Enough (sequence, KV head) items for the plans that share whole items."""
+    require_shared_plans()
+    heads, window, sinks = HEADS[0], 255, 20
+    lens = [300 + 37 * (i % 29) for i in range(300)]
+    meta, pool, scales, q = make(gpu, [n - 1 for n in lens], [1] * len(lens), heads,
+                                 torch.bfloat16, False, window, sinks, seed=5)
+    w = plan_decode(gpu, meta, heads, torch.bfloat16, window, sinks, kind)
+    assert w.plan_kind == {"host": "shared", "device": "device_shared"}[kind]
+    out, lse = w.run(q, pool, return_lse=True)
+    rows = list(range(0, len(lens), 7))
+    ref = reference(meta, pool, scales, q, window, sinks, b_rows=set(rows))
+    check(out, lse, ref, rows)
+    if kind == "device":
+        w.update_plan()
+        again, lse2 = w.run(q, pool, return_lse=True)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
+def test_decode_long_window(gpu):
+    """A long sequence on its own: its window is cut over the GPU and merged."""
+    heads, window, sinks = HEADS[1], 9000, 64
+    for kind in ("host", "device"):
+        meta, pool, scales, q = make(gpu, [30000], [1], heads, torch.bfloat16, False, window,
+                                     sinks, seed=9, spoil=False)
+        w = plan_decode(gpu, meta, heads, torch.bfloat16, window, sinks, kind)
+        out, lse = w.run(q, pool, return_lse=True)
+        check(out, lse, reference(meta, pool, scales, q, window, sinks))
+
+
+@pytest.mark.parametrize("kind", ["host", "whole", "device"])
+@pytest.mark.parametrize("batch", [9, 300])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_fused_append_is_the_separate_calls(gpu, kind, batch, fp8):
+    """RoPE + append + windowed attention in one call: the bits of the three."""
+    heads, window, sinks, dtype = HEADS[0], 100, 20, torch.bfloat16
+    hq, hkv, d = heads
+    lens = [LENS[i % len(LENS)] + 16 * (i % 5) for i in range(batch)]
+    meta, pool, scales, q = make(gpu, [n - 1 for n in lens], [1] * batch, heads, dtype, fp8,
+                                 window, sinks, seed=3)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(4)
+    k, v = (torch.randn((batch, hkv, d), generator=g, device=gpu).to(dtype) for _ in range(2))
+    lists = [i32(x, gpu) for x in (meta.kv_indices, meta.kv_indptr, meta.kv_last_page_len)]
+    bi, pos = i32(np.arange(batch), gpu), i32(np.asarray(lens) - 1, gpu)
+    for rope in (None, (2.0, 10000.0)):
+        p1, p2 = pool.clone(), pool.clone()
+        q1, k1 = q.clone(), k.clone()
+        if rope:
+            pagedattn.apply_rope_pos_ids_inplace(q1, k1, pos, rope_scale=rope[0],
+                                                 rope_theta=rope[1])
+        pagedattn.append_paged_kv_cache(k1, v, bi, pos, p1, *lists, kv_layout="HND",
+                                        kv_scales=scales)
+        w = plan_decode(gpu, meta, heads, dtype, window, sinks, kind)
+        want = w.run(q1, p1, kv_scales=scales)
+        got = w.run(q, p2, kv_scales=scales, append_key=k, append_value=v, rope=rope,
+                    positions=pos if rope and kind == "host" else None)
+        assert torch.equal(p1.view(torch.uint8), p2.view(torch.uint8))
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["host", "device"])
+def test_window_past_the_length_is_no_window(gpu, kind):
+    heads, dtype = HEADS[1], torch.bfloat16
+    meta, pool, scales, q = make(gpu, [n - 1 for n in LENS], [1] * len(LENS), heads, dtype,
+                                 False, 1 << 30, 0, seed=2)
+    w = plan_decode(gpu, meta, heads, dtype, 1 << 30, 0, kind)
+    assert torch.equal(w.run(q, pool), plan_decode(gpu, meta, heads, dtype, -1, 0, kind)
+                       .run(q, pool))
+
+
+def plan_prefill(device, meta, heads, dtype, window, sinks, device_plan, causal=True):
+    w = pagedattn.BatchPrefillWithPagedKVCacheWrapper(workspace(device), "HND")
+    w.plan(i32(meta.qo_indptr, device), i32(meta.kv_indptr, device), i32(meta.kv_indices, device),
+           i32(meta.kv_last_page_len, device), *heads, 16, causal=causal, q_data_type=dtype,
+           window_left=window, num_sink_tokens=sinks, device_plan=device_plan,
+           max_qo_tokens=meta.nnz)
+    return w
+
+
+CHUNKS = [([0, 5, 300, 0, 77], [1, 40, 70, 200, 0]), ([1500], [33]), ([0], [400])]
+
+
+@pytest.mark.parametrize("computed,chunks", CHUNKS)
+@pytest.mark.parametrize("window,sinks", [(127, 4), (0, 0), (16, 17), (63, 130), (100000, 3)])
+@pytest.mark.parametrize("heads,dtype,fp8", [
+    (HEADS[0], torch.float16, False), (HEADS[1], torch.bfloat16, False),
+    (HEADS[1], torch.bfloat16, True), (HEADS[2], torch.float16, True),
+    (HEADS[3], torch.bfloat16, False)])
+def test_prefill(gpu, heads, dtype, fp8, window, sinks, computed, chunks):
+    meta, pool, scales, q = make(gpu, computed, chunks, heads, dtype, fp8, window, sinks,
+                                 seed=window + sinks)
+    got = []
+    for device_plan in (False, True):
+        w = plan_prefill(gpu, meta, heads, dtype, window, sinks, device_plan)
+        got.append(w.run(q, pool, kv_scales=scales, return_lse=True))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    rows = sorted({0, 1, meta.nnz - 1, *range(0, meta.nnz, 13)} & set(range(meta.nnz)))
+    check(*got[0], reference(meta, pool, scales, q, window, sinks, b_rows=set(rows)), rows)
+
+
+@pytest.mark.parametrize("heads,dtype,fp8", [(HEADS[1], torch.bfloat16, False),
+                                             (HEADS[0], torch.float16, True)])
+def test_prefill_cut_windows(gpu, heads, dtype, fp8, monkeypatch):
+    """A long window of few rows runs in pieces and is merged; whole, it is the same within the
+    bound."""
+    window, sinks = 4000, 200
+    meta, pool, scales, q = make(gpu, [9000], [64], heads, dtype, fp8, window, sinks, seed=1,
+                                 spoil=False)
+    rows = [0, 31, 63]
+    ref = reference(meta, pool, scales, q, window, sinks, b_rows=set(rows))
+    for env in ("1", "0"):
+        monkeypatch.setenv("PAGEDATTN_PREFILL_SPLIT", env)
+        for device_plan in (False, True):
+            w = plan_prefill(gpu, meta, heads, dtype, window, sinks, device_plan)
+            check(*w.run(q, pool, kv_scales=scales, return_lse=True), ref, rows)
+
+
+def test_prefill_not_causal(gpu):
+    heads, dtype, window, sinks = HEADS[1], torch.bfloat16, 20, 3
+    meta, pool, scales, q = make(gpu, [100, 0], [50, 90], heads, dtype, False, window, sinks,
+                                 seed=1)
+    w = plan_prefill(gpu, meta, heads, dtype, window, sinks, False, causal=False)
+    check(*w.run(q, pool, return_lse=True),
+          reference(meta, pool, scales, q, window, sinks, causal=False))
+
+
+def test_prefill_rows_that_see_nothing(gpu):
+    """More query rows than tokens: the rows before the first token are zeros."""
+    heads, dtype, window, sinks = HEADS[0], torch.float16, 9, 2
+    meta, pool, scales, q = make(gpu, [0], [60], heads, dtype, False, window, sinks, seed=1,
+                                 spoil=False)
+    meta.kv_indptr[1:] = 2  # 2 pages, the last of 5 tokens
+    meta.kv_last_page_len[0] = 5
+    w = plan_prefill(gpu, meta, heads, dtype, window, sinks, False)
+    out, lse = w.run(q, pool, return_lse=True)
+    check(out, lse, reference(meta, pool, scales, q, window, sinks))
+    assert not out[:60 - 21].any() and bool(torch.isneginf(lse[:60 - 21]).all())
+
+
+@pytest.mark.parametrize("heads,fp8", [(HEADS[0], False), (HEADS[1], False), (HEADS[1], True)])
+@pytest.mark.parametrize("long", [False, True])
+def test_prefill_tokens_not_finite_reach_the_rows_that_see_them_only(gpu, heads, fp8, long):
+    """An infinity and a NaN that some rows of a tile see: those rows are not finite as in the
+    reference, all others are as if the tokens were not there."""
+    dtype, window, sinks = torch.bfloat16, 30, 2
+    prefix = 2000 if long else 40
+    window = 1500 if long else window
+    meta, pool, scales, q = make(gpu, [prefix], [150], heads, dtype, fp8, window, sinks, seed=8)
+    table = meta.kv_indices[meta.kv_indptr[0]:]
+    for t, x in ((prefix + 60, math.nan), (prefix - window + 20, math.nan if fp8 else math.inf)):
+        pool[table[t // 16], 1, :, t % 16] = x
+    seen = [r for r in range(150) if any(
+        t <= prefix + r and t >= prefix + r - window for t in (prefix + 60, prefix - window + 20))]
+    clear = sorted(set(range(150)) - set(seen))
+    assert len(clear) > 20 and len(seen) > 20
+    w = plan_prefill(gpu, meta, heads, dtype, window, sinks, False)
+    out, lse = w.run(q, pool, kv_scales=scales, return_lse=True)
+    check(out, lse, reference(meta, pool, scales, q, window, sinks, b_rows=set(clear)), clear)
+    assert not bool(torch.isfinite(out[seen]).any())
+
+
+def test_decode_step_replayed_from_a_graph(gpu):
+    """Metadata, plan and fused windowed decode captured once; lengths, rows and tables change
+    in place between replays, with eager work between them."""
+    heads, window, sinks, dtype, batch = HEADS[0], 70, 17, torch.float16, 5
+    hq, hkv, d = heads
+    rng = np.random.default_rng(0)
+    tables = rng.permutation(batch * 30).reshape(batch, 30)
+    bt, lens = i32(tables, gpu), i32(np.ones(batch), gpu)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(0)
+    pool = torch.randn((batch * 30, 2, hkv, 16, d), generator=g, device=gpu).to(dtype)
+    q = torch.zeros((batch, hq, d), dtype=dtype, device=gpu)
+    k, v = (torch.zeros((batch, hkv, d), dtype=dtype, device=gpu) for _ in range(2))
+    out = torch.zeros_like(q)
+    for with_update in (False, True):
+        buf = pagedattn.ops.new_paged_buffers(batch, batch * 30, batch, gpu)
+        w = pagedattn.BatchDecodeWithPagedKVCacheWrapper(
+            workspace(gpu), "HND", use_cuda_graph=True, paged_kv_indptr_buffer=buf.kv_indptr,
+            paged_kv_indices_buffer=buf.kv_indices,
+            paged_kv_last_page_len_buffer=buf.kv_last_page_len)
+        w.plan(buf.kv_indptr, buf.kv_indices, buf.kv_last_page_len, hq, hkv, d, 16,
+               q_data_type=dtype, window_left=window, num_sink_tokens=sinks)
+
+        def step():
+            pagedattn.build_paged_metadata(bt, lens, out=buf)
+            if with_update:
+                w.update_plan()
+            w.run(q, pool, out=out, append_key=k, append_value=v, rope=(1.0, 10000.0),
+                  positions=buf.positions)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for i, now in enumerate(([1, 17, 90, 300, 64], [2, 18, 91, 301, 65], [480, 3, 5, 86, 88])):
+            lens.copy_(i32(now, gpu))
+            for x in (q, k, v):
+                x.normal_(generator=g)
+            before = pool.clone()
+            graph.replay()
+            torch.cuda.synchronize()
+            got, wrote = out.clone(), pool.clone()
+            pool.copy_(before)
+            meta = decode_metadata([t.tolist() for t in tables], now)
+            we = plan_decode(gpu, meta, heads, dtype, window, sinks, "device")
+            want = we.run(q, pool, append_key=k, append_value=v, rope=(1.0, 10000.0))
+            assert torch.equal(got, want), i
+            assert torch.equal(wrote, pool), i
