@@ -199,6 +199,92 @@ int pagedattn_fork_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layers,
                          const int32_t* dst_pages, const int32_t* valid_tokens,
                          int32_t num_forks, int32_t* error_flag, void* stream);
 
+/* Page tables kept on the device.  block_tables: [batch_size, table_stride]
+ * int32, the first max_pages entries of row b are sequence b's pages, -1 where
+ * there is none; ref_counts [num_pages] int32: the table entries (and other
+ * holders) of each page, 0 for a free one.  All of it is graph-capturable and
+ * nothing is copied to the host.  *error_flag (int32, optional) is incremented
+ * once per row or entry that names a page outside the pool or does not fit
+ * its table; such rows and entries are skipped.
+ *
+ * pagedattn_reserve_pages: kv_lens[b] counts the step's new_lens[b] tokens (NULL:
+ * one per sequence) already.  Every slot they open gets a free page (count
+ * 1), lowest ids first in (row, slot) order.  A partial page that the tokens
+ * continue and that others hold is forked first: a free page takes its rows in
+ * every layer and its place in the table, and its count drops by one; of
+ * several rows that continue one page, the last keeps it if nothing
+ * else holds it.  Where the free pages do not suffice, nothing is changed and
+ * error_flag[1] (error_flag holds two int32 here) grows by the pages missing.
+ * pagedattn_release_pages: the rows' slots [first_slots[b], last_slots[b]) (NULL:
+ * 0, max_pages) are emptied and their pages' counts drop by one each; an entry
+ * whose page's count is 0 already counts as an error.
+ * pagedattn_release_window_pages: the same for the pages that lie wholly between
+ * the sinks and the window of the token at kv_lens[b] - 1 (see
+ * pagedattn_decode_window_metadata): no later token sees them.
+ * pagedattn_share_pages: row dst_rows[i] is set to row src_rows[i]'s pages and
+ * length, whose counts grow by one (the entries it had are not released).  A
+ * destination that is a source or another one's destination is skipped and
+ * counted.
+ * pagedattn_compact_pages: the n pages with a count move to ids [0, n) in every
+ * layer (those there already stay), with their counts and the entries that name
+ * them; remap [num_pages] int32 gets each page's new id, -1 for free ones, for
+ * tables kept elsewhere.
+ * scratch: pagedattn_page_scratch_bytes device bytes, 256-byte aligned, for the
+ * call alone. */
+size_t pagedattn_page_scratch_bytes(int32_t num_pages, int32_t batch_size, int32_t max_pages);
+int pagedattn_reserve_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layers,
+                            int32_t num_pages, int32_t num_kv_heads, int32_t head_dim,
+                            int32_t page_size, float* kv_scales, int32_t* block_tables,
+                            int64_t table_stride, int32_t max_pages, const int32_t* kv_lens,
+                            const int32_t* new_lens, int32_t batch_size, int32_t* ref_counts,
+                            int32_t* error_flag, void* scratch, size_t scratch_bytes,
+                            void* stream);
+int pagedattn_release_pages(int32_t* block_tables, int64_t table_stride, int32_t max_pages,
+                            int32_t batch_size, int32_t* ref_counts, int32_t num_pages,
+                            const int32_t* first_slots, const int32_t* last_slots,
+                            int32_t* error_flag, void* stream);
+int pagedattn_release_window_pages(int32_t* block_tables, int64_t table_stride, int32_t max_pages,
+                                   const int32_t* kv_lens, int32_t batch_size,
+                                   int32_t* ref_counts, int32_t num_pages, int32_t window_left,
+                                   int32_t sinks, int32_t* error_flag, void* stream);
+int pagedattn_share_pages(int32_t* block_tables, int64_t table_stride, int32_t max_pages,
+                          int32_t* kv_lens, int32_t batch_size, const int32_t* src_rows,
+                          const int32_t* dst_rows, int32_t num_shares, int32_t* ref_counts,
+                          int32_t num_pages, int32_t* error_flag, void* stream);
+int pagedattn_compact_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layers,
+                            int32_t num_pages, int32_t num_kv_heads, int32_t head_dim,
+                            int32_t page_size, float* kv_scales, int32_t* block_tables,
+                            int64_t table_stride, int32_t max_pages, int32_t batch_size,
+                            int32_t* ref_counts, int32_t* remap, int32_t* error_flag,
+                            void* scratch, size_t scratch_bytes, void* stream);
+
+/* RoPE whose frequencies turn by the positions of several axes (time, height and
+ * width of tokens of images and videos), in place on q and k; and the same with
+ * the page append of the k and v rows.  axis_positions: [num_axes, nnz]
+ * int32 (device), rows axis_stride apart; sections [num_axes] (host): how many
+ * of the rotary_dim / 2 frequencies each axis turns.  Blocks: the axes take
+ * theirs one after the other.  cyclic != 0: frequency i goes to axis
+ * a = i mod num_axes while i < num_axes * sections[a], and to axis 0 beyond.
+ * rotary_dim (0: head_dim) and head_dim are multiples of 16; elements past
+ * rotary_dim are not turned.  batch_indices, positions and the cache are those of
+ * pagedattn_append_paged_kv_cache: positions are places in the cache. */
+int pagedattn_apply_multi_axis_rope_inplace(
+    void* q, void* k, const int32_t* axis_positions, int64_t axis_stride, int32_t num_axes,
+    const int32_t* sections, int32_t cyclic, int32_t nnz, int32_t num_qo_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim, int64_t q_stride_n,
+    int64_t q_stride_h, int64_t k_stride_n, int64_t k_stride_h, int32_t interleave,
+    float rope_scale, float rope_theta, int32_t dtype, void* stream);
+int pagedattn_multi_axis_rope_append_paged_kv_cache(
+    void* q, int64_t q_stride_n, int64_t q_stride_h, int32_t num_qo_heads, void* append_key,
+    const void* append_value, int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n,
+    int64_t v_stride_h, int32_t src_dtype, const int32_t* axis_positions, int64_t axis_stride,
+    int32_t num_axes, const int32_t* sections, int32_t cyclic, const int32_t* batch_indices,
+    const int32_t* positions, int32_t nnz, int32_t rotary_dim, int32_t interleave,
+    float rope_scale, float rope_theta, void* paged_kv_cache, int32_t cache_dtype,
+    const float* kv_scales, int32_t num_pages, const int32_t* kv_indices, int32_t num_indices,
+    const int32_t* kv_indptr, int32_t batch_size, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, int32_t* error_flag, void* stream);
+
 /* Step metadata built on the device (replaces the Python list building and
  * upload of src/engine/runtime/step_executor.py:98-165 (prefill) and
  * :204-234 (decode), and the device-to-host sync of

@@ -39,6 +39,25 @@ __device__ __forceinline__ int64_t append_target_page(const AppendArgs& a,
   return page;
 }
 
+// Writes one 8-element chunk of a K (kind 0) or V (kind 1) row of head h to
+// slot `slot` of `page`.  e4m3 pools: quantised with the page's fixed scale
+// (quant8_e4m3); a clamped chunk is counted in a.err[1].
+template <bool IS_BF16, bool TO_FP8>
+__device__ __forceinline__ void store_chunk(const AppendArgs& a, int64_t page, int slot,
+                                            int kind, int h, int d0, u32x4 x) {
+  const int64_t dst_elem =
+      (((page * 2 + kind) * a.hkv + h) * kPage + slot) * (int64_t)a.d + d0;
+  if constexpr (!TO_FP8) {
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.cache) + dst_elem) = x;
+  } else {
+    const float scale = a.scales[(page * 2 + kind) * a.hkv + h];
+    bool clamped = false;
+    const u32x2 o = quant8_e4m3<IS_BF16>(x, scale, &clamped);
+    *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.cache) + dst_elem) = o;
+    count_lanes(a.err ? a.err + 1 : nullptr, clamped);
+  }
+}
+
 // Validation and argument packing shared by the append entry points.
 // Returns PAGEDATTN_OK with *a filled, or an error; *empty is set when there
 // is nothing to do (nnz == 0).

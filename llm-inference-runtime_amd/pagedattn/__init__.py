@@ -12,14 +12,21 @@ from .ops import (  # noqa: F401
     BatchPrefillWithPagedKVCacheWrapper,
     append_paged_kv_cache,
     append_paged_kv_cache_e4m3_amax,
+    apply_multi_axis_rope_inplace,
     apply_rope_pos_ids_inplace,
     build_paged_metadata,
+    compact_pages,
     copy_bytes,
     fork_pages,
     get_batch_indices_positions,
+    multi_axis_rope_append_paged_kv_cache,
     quantize_pages_e4m3,
     read_bytes,
+    release_pages,
+    release_window_pages,
+    reserve_pages,
     rope_append_paged_kv_cache,
+    share_pages,
 )
 from ._lib import LIB_PATH, PagedAttnError, lib  # noqa: F401
 
@@ -29,14 +36,21 @@ __all__ = [
     "BatchPrefillWithPagedKVCacheWrapper",
     "append_paged_kv_cache",
     "append_paged_kv_cache_e4m3_amax",
+    "apply_multi_axis_rope_inplace",
     "apply_rope_pos_ids_inplace",
     "build_paged_metadata",
+    "compact_pages",
     "copy_bytes",
     "fork_pages",
     "get_batch_indices_positions",
+    "multi_axis_rope_append_paged_kv_cache",
     "quantize_pages_e4m3",
     "read_bytes",
+    "release_pages",
+    "release_window_pages",
+    "reserve_pages",
     "rope_append_paged_kv_cache",
+    "share_pages",
     "LIB_PATH",
     "PagedAttnError",
     "lib",

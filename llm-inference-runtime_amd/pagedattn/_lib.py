@@ -73,6 +73,33 @@ _SIGNATURES = {
         _c_int,
         [_c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_int,
          _c_p, _c_p]),
+    "pagedattn_page_scratch_bytes": (_c_sz, [_c_int, _c_int, _c_int]),
+    "pagedattn_reserve_pages": (
+        _c_int,
+        [_c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_i64, _c_int, _c_p,
+         _c_p, _c_int, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "pagedattn_release_pages": (
+        _c_int, [_c_p, _c_i64, _c_int, _c_int, _c_p, _c_int, _c_p, _c_p, _c_p, _c_p]),
+    "pagedattn_release_window_pages": (
+        _c_int,
+        [_c_p, _c_i64, _c_int, _c_p, _c_int, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p]),
+    "pagedattn_share_pages": (
+        _c_int,
+        [_c_p, _c_i64, _c_int, _c_p, _c_int, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p]),
+    "pagedattn_compact_pages": (
+        _c_int,
+        [_c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_i64, _c_int, _c_int,
+         _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "pagedattn_apply_multi_axis_rope_inplace": (
+        _c_int,
+        [_c_p, _c_p, _c_p, _c_i64, _c_int, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_f, _c_f, _c_int, _c_p]),
+    "pagedattn_multi_axis_rope_append_paged_kv_cache": (
+        _c_int,
+        [_c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_p, _c_i64, _c_int, _c_p, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_f, _c_f,
+         _c_p, _c_int, _c_p, _c_int, _c_p, _c_int, _c_p, _c_int, _c_int, _c_int, _c_int, _c_p,
+         _c_p]),
     "pagedattn_plan_create": (_c_p, []),
     "pagedattn_plan_destroy": (None, [_c_p]),
     "pagedattn_decode_plan": (

@@ -28,6 +28,7 @@ scales as pages fill) and ``fork_pages`` (copy-on-write page fork).
 
 from __future__ import annotations
 
+import ctypes
 import math
 import operator
 from dataclasses import dataclass
@@ -307,6 +308,111 @@ def rope_append_paged_kv_cache(q: torch.Tensor, append_key: torch.Tensor,
          ptr(indptr), bsz, hkv, d, PAGE_SIZE, ptr(error_flag), _stream(device))
 
 
+def _on(device: torch.device, name: str, *args) -> None:
+    """Entry point `name` on `device` and its current stream, whichever device
+    is current."""
+    if device.index in (None, torch.cuda.current_device()):
+        call(name, *args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _stream(device))
+
+
+def _axes(axis_positions: torch.Tensor, sections, nnz: int, device: torch.device,
+          rope_scale: float, rope_theta: float):
+    """The axis arguments of a multi-axis call: positions, their row stride, the
+    sections as C ints."""
+    _require_cuda(axis_positions, "axis_positions")
+    if axis_positions.dim() != 2 or axis_positions.shape[1] != nnz:
+        raise ValueError(f"axis_positions must be [axes, {nnz}], got "
+                         f"{tuple(axis_positions.shape)}")
+    if axis_positions.dtype.is_floating_point or axis_positions.dtype.is_complex:
+        raise ValueError("axis_positions must be whole numbers")
+    shares = [operator.index(x) for x in sections]
+    if len(shares) != axis_positions.shape[0]:
+        raise ValueError(f"{len(shares)} sections for {axis_positions.shape[0]} axes")
+    if any(x < 0 or x >= 1 << 31 for x in shares):
+        raise ValueError(f"sections {shares} must not be negative")
+    for name, x in (("rope_scale", rope_scale), ("rope_theta", rope_theta)):
+        if not (x > 0 and math.isfinite(x)):
+            raise ValueError(f"{name} must be positive and finite")
+    pos = axis_positions.to(device=device, dtype=torch.int32)
+    if pos.stride(1) != 1 or pos.stride(0) < nnz:
+        pos = pos.contiguous()
+    return pos, max(pos.stride(0), nnz), (ctypes.c_int32 * len(shares))(*shares)
+
+
+def apply_multi_axis_rope_inplace(q: torch.Tensor, k: torch.Tensor, axis_positions: torch.Tensor,
+                                  sections, cyclic: bool = False, rotary_dim: int | None = None,
+                                  interleave: bool = False, rope_scale: float = 1.0,
+                                  rope_theta: float = 1e4) -> None:
+    """RoPE in place on q [nnz, Hq, D] and k [nnz, Hkv, D] whose frequencies turn
+    by the positions of several axes, axis_positions [axes, nnz] (1 to 4 axes:
+    time, height and width of tokens of images and videos).
+
+    Frequency i of the rotary_dim / 2 turns by axis_positions[a, t] / rope_scale
+    * rope_theta ** (-2 i / rotary_dim).  sections: how many frequencies each
+    axis turns.  They take theirs one after the other; with cyclic=True
+    frequency i goes to axis a = i mod axes while i < axes * sections[a], and
+    to axis 0 beyond.  Pairs are half of rotary_dim apart, or adjacent
+    (interleave).  With equal positions on all axes this is
+    apply_rope_pos_ids_inplace, bit for bit."""
+    _check_rows(q, "q", None, None)
+    _check_rows(k, "k", None, q.shape[2])
+    if q.dtype != k.dtype or q.device != k.device:
+        raise ValueError("q and k must share a dtype and a device")
+    nnz, hq, d = q.shape
+    if k.shape[0] != nnz:
+        raise ValueError("q and k must have the same number of tokens")
+    pos, stride, shares = _axes(axis_positions, sections, nnz, q.device, rope_scale, rope_theta)
+    _on(q.device, "pagedattn_apply_multi_axis_rope_inplace", ptr(q), ptr(k), ptr(pos), stride,
+        len(shares), shares, int(bool(cyclic)), nnz, hq, k.shape[1], d, int(rotary_dim or d),
+        q.stride(0), q.stride(1), k.stride(0), k.stride(1), int(bool(interleave)),
+        float(rope_scale), float(rope_theta), dtype_code(q.dtype))
+
+
+def multi_axis_rope_append_paged_kv_cache(
+        q: torch.Tensor, append_key: torch.Tensor, append_value: torch.Tensor,
+        axis_positions: torch.Tensor, sections, batch_indices: torch.Tensor,
+        positions: torch.Tensor, paged_kv_cache: torch.Tensor, kv_indices: torch.Tensor,
+        kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor, kv_layout: str = "NHD",
+        rope_scale: float = 1.0, rope_theta: float = 1e4, cyclic: bool = False,
+        rotary_dim: int | None = None, interleave: bool = False,
+        kv_scales: torch.Tensor | None = None, error_flag: torch.Tensor | None = None) -> None:
+    """apply_multi_axis_rope_inplace(q, append_key, axis_positions, ...) followed
+    by append_paged_kv_cache(...) in one launch, with the results of the two.
+    `positions` are the tokens' places in the cache, which the axis positions of
+    images and of text after them differ from."""
+    num_pages, hkv, d = _check_pool(paged_kv_cache, None, None, kv_layout)
+    _check_rows(q, "q", None, d)
+    _check_rows(append_key, "append_key", hkv, d)
+    _check_rows(append_value, "append_value", hkv, d)
+    if not (q.dtype == append_key.dtype == append_value.dtype):
+        raise ValueError("q, append_key and append_value must share a dtype")
+    device = paged_kv_cache.device
+    if not (q.device == append_key.device == append_value.device == device):
+        raise ValueError("q, append_key, append_value and the pool must be on one device")
+    nnz = append_key.shape[0]
+    if (q.shape[0] != nnz or append_value.shape[0] != nnz or batch_indices.numel() != nnz
+            or positions.numel() != nnz):
+        raise ValueError("q, append_key/value, batch_indices and positions disagree on nnz")
+    scales = _check_scales(kv_scales, paged_kv_cache)
+    if paged_kv_cache.dtype not in (append_key.dtype, torch.float8_e4m3fn):
+        raise ValueError(f"pool dtype {paged_kv_cache.dtype} cannot take {append_key.dtype} rows")
+    pos, stride, shares = _axes(axis_positions, sections, nnz, device, rope_scale, rope_theta)
+    bi, at = _i32(batch_indices, device), _i32(positions, device)
+    ind, indptr = _i32(kv_indices, device), _i32(kv_indptr, device)
+    _check_error_flag(error_flag, 2 if paged_kv_cache.dtype == torch.float8_e4m3fn else 1)
+    _on(device, "pagedattn_multi_axis_rope_append_paged_kv_cache", ptr(q), q.stride(0),
+        q.stride(1), q.shape[1], ptr(append_key), ptr(append_value), append_key.stride(0),
+        append_key.stride(1), append_value.stride(0), append_value.stride(1),
+        dtype_code(append_key.dtype), ptr(pos), stride, len(shares), shares, int(bool(cyclic)),
+        ptr(bi), ptr(at), nnz, int(rotary_dim or d), int(bool(interleave)), float(rope_scale),
+        float(rope_theta), ptr(paged_kv_cache), dtype_code(paged_kv_cache.dtype), ptr(scales),
+        num_pages, ptr(ind), ind.numel(), ptr(indptr), indptr.numel() - 1, hkv, d, PAGE_SIZE,
+        ptr(error_flag))
+
+
 def append_paged_kv_cache_e4m3_amax(append_key: torch.Tensor, append_value: torch.Tensor,
                                     batch_indices: torch.Tensor, positions: torch.Tensor,
                                     paged_kv_cache: torch.Tensor, kv_indices: torch.Tensor,
@@ -357,6 +463,188 @@ def append_paged_kv_cache_e4m3_amax(append_key: torch.Tensor, append_value: torc
          append_value.stride(1), dtype_code(append_key.dtype), ptr(bi), ptr(pos), nnz,
          ptr(paged_kv_cache), ptr(scales), num_pages, ptr(ind), ind.numel(), ptr(indptr), bsz,
          hkv, d, PAGE_SIZE, ptr(error_flag), _stream(device))
+
+
+def _whole_pool(kv_pool: torch.Tensor, kv_scales: torch.Tensor | None):
+    """(layers, pages, Hkv, D, scales) of the engine's pool of all layers."""
+    _require_cuda(kv_pool, "kv_pool")
+    if kv_pool.dim() != 6 or kv_pool.shape[2] != 2 or kv_pool.shape[4] != PAGE_SIZE:
+        raise ValueError("kv_pool must be [L, num_pages, 2, num_kv_heads, 16, head_dim], "
+                         f"got {tuple(kv_pool.shape)}")
+    if not kv_pool.is_contiguous():
+        raise ValueError("kv_pool must be contiguous")
+    n_layers, num_pages, _, hkv, _, d = kv_pool.shape
+    if kv_pool.dtype != torch.float8_e4m3fn:
+        return n_layers, num_pages, hkv, d, None
+    if kv_scales is None:
+        raise ValueError("an e4m3 pool needs kv_scales [L, num_pages, 2, num_kv_heads]")
+    if (kv_scales.dtype != torch.float32 or not kv_scales.is_contiguous()
+            or tuple(kv_scales.shape) != (n_layers, num_pages, 2, hkv)
+            or kv_scales.device != kv_pool.device):
+        raise ValueError(f"kv_scales must be contiguous float32 [{n_layers}, {num_pages}, "
+                         f"2, {hkv}] on the pool's device, got {kv_scales.dtype} "
+                         f"{tuple(kv_scales.shape)}")
+    return n_layers, num_pages, hkv, d, kv_scales
+
+
+def _page_tables(block_tables: torch.Tensor, ref_counts: torch.Tensor, num_pages: int | None,
+                 error_flag: torch.Tensor | None, flags: int, **ints) -> torch.device:
+    """Checks the tables, counts and per-row int32 tensors of the page calls."""
+    _require_cuda(block_tables, "block_tables")
+    device = block_tables.device
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.numel() and (
+            (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)
+            or (block_tables.shape[0] > 1 and block_tables.stride(0) < block_tables.shape[1])):
+        raise ValueError("block_tables must be an int32 [batch, max_pages] tensor with "
+                         "contiguous rows")
+    for name, t, n in [("ref_counts", ref_counts, num_pages),
+                       *((k, *v) for k, v in ints.items())]:
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or \
+                not t.is_contiguous() or (n is not None and t.numel() != n):
+            size = "" if n is None else f" of {n} entries"
+            raise ValueError(f"{name} must be a contiguous int32 tensor{size} on "
+                             "block_tables' device")
+    _check_error_flag(error_flag, flags)
+    if error_flag is not None and error_flag.device != device:
+        raise ValueError("error_flag must be on block_tables' device")
+    return device
+
+
+def _row_stride(block_tables: torch.Tensor) -> int:
+    return max(block_tables.stride(0), block_tables.shape[1])
+
+
+def _page_scratch(device: torch.device, num_pages: int, block_tables: torch.Tensor):
+    n = _lib.lib().pagedattn_page_scratch_bytes(num_pages, *block_tables.shape)
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def reserve_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor,
+                  new_lens: torch.Tensor | None, ref_counts: torch.Tensor,
+                  kv_scales: torch.Tensor | None = None,
+                  error_flag: torch.Tensor | None = None) -> None:
+    """Pages for a step's new tokens, taken and forked on the device.
+
+    block_tables [B, max_pages] (-1: no page), kv_lens [B] (the step's
+    new_lens[b] tokens counted already, as in build_paged_metadata; None: one
+    each) and ref_counts [num_pages] are int32 device tensors; tables and counts
+    are updated in place.  Every slot that the new tokens open gets a free
+    page (count 0 -> 1), the lowest ids first, in row and slot order.  A
+    partial page that the tokens continue while others hold it is forked
+    (todo.md:17-19): a free page takes its rows in every layer of kv_pool [L, P,
+    2, Hkv, 16, D] (and of kv_scales for an e4m3 pool) and its place in the
+    table; of several rows that continue one page the last keeps it, if nothing
+    else holds it.
+
+    error_flag (two int32, optional): [0] grows by the rows that were skipped
+    because their lengths do not fit their table or their partial page is none of
+    the pool's held ones; where the free pages do not suffice, nothing is changed
+    and [1] grows by the pages missing."""
+    n_layers, num_pages, hkv, d, scales = _whole_pool(kv_pool, kv_scales)
+    bsz, max_pages = block_tables.shape if block_tables.dim() == 2 else (0, 0)
+    device = _page_tables(block_tables, ref_counts, num_pages, error_flag, 2,
+                          kv_lens=(kv_lens, bsz), new_lens=(new_lens, bsz))
+    if kv_pool.device != device:
+        raise ValueError("kv_pool and block_tables must be on one device")
+    scratch = _page_scratch(device, num_pages, block_tables)
+    _on(device, "pagedattn_reserve_pages", ptr(kv_pool), dtype_code(kv_pool.dtype), n_layers,
+        num_pages, hkv, d, PAGE_SIZE, ptr(scales), ptr(block_tables), _row_stride(block_tables),
+        max_pages, ptr(kv_lens), ptr(new_lens), bsz, ptr(ref_counts), ptr(error_flag),
+        ptr(scratch), scratch.numel())
+
+
+def release_pages(block_tables: torch.Tensor, ref_counts: torch.Tensor,
+                  first_slots: torch.Tensor | None = None,
+                  last_slots: torch.Tensor | None = None,
+                  error_flag: torch.Tensor | None = None) -> None:
+    """Slots [first_slots[b], last_slots[b]) of every row of block_tables (None: from
+    0, to the row's end) are emptied (-1) and their pages' counts drop by one;
+    a page is free when its count is 0.  Empty slots are passed over.
+    error_flag counts entries outside the pool, and those whose page's count was
+    0 already."""
+    bsz = block_tables.shape[0] if block_tables.dim() else 0
+    device = _page_tables(block_tables, ref_counts, None, error_flag, 1,
+                          first_slots=(first_slots, bsz), last_slots=(last_slots, bsz))
+    _on(device, "pagedattn_release_pages", ptr(block_tables), _row_stride(block_tables),
+        block_tables.shape[1], bsz, ptr(ref_counts), ref_counts.numel(), ptr(first_slots),
+        ptr(last_slots), ptr(error_flag))
+
+
+def release_window_pages(block_tables: torch.Tensor, kv_lens: torch.Tensor,
+                         ref_counts: torch.Tensor, window_left: int, num_sink_tokens: int = 0,
+                         error_flag: torch.Tensor | None = None) -> None:
+    """release_pages of the pages that lie wholly behind the window of the token
+    at kv_lens[b] - 1 and past the sinks: neither it nor any later token sees
+    them, and the windowed attention calls do not read their entries."""
+    left, sinks = _window(window_left, num_sink_tokens)
+    if left < 0:
+        raise ValueError("release_window_pages needs a window (window_left >= 0)")
+    bsz = block_tables.shape[0] if block_tables.dim() else 0
+    device = _page_tables(block_tables, ref_counts, None, error_flag, 1, kv_lens=(kv_lens, bsz))
+    _on(device, "pagedattn_release_window_pages", ptr(block_tables), _row_stride(block_tables),
+        block_tables.shape[1], ptr(kv_lens), bsz, ptr(ref_counts), ref_counts.numel(), left, sinks,
+        ptr(error_flag))
+
+
+def share_pages(block_tables: torch.Tensor, kv_lens: torch.Tensor, src_rows, dst_rows,
+                ref_counts: torch.Tensor, error_flag: torch.Tensor | None = None) -> None:
+    """Row dst_rows[i] of block_tables becomes a second holder of row src_rows[i]'s
+    pages, with its length (parallel samples of one prompt, beams): the counts
+    of those pages grow by one and reserve_pages forks the partial one when
+    either row goes on.  What the destination row held is overwritten, not
+    released.
+
+    Row lists given on the host are checked here (in range, destinations distinct
+    and not among the sources); device tensors are checked in the kernel,
+    which skips a bad share and counts it in `error_flag`."""
+    bsz = block_tables.shape[0] if block_tables.dim() else 0
+    device = _page_tables(block_tables, ref_counts, None, error_flag, 1, kv_lens=(kv_lens, bsz))
+    rows = []
+    host = []
+    for name, x in (("src_rows", src_rows), ("dst_rows", dst_rows)):
+        if isinstance(x, torch.Tensor) and x.device.type == "cuda":
+            rows.append(_i32(x.reshape(-1), device))
+            continue
+        h = torch.as_tensor(x, dtype=torch.int64).reshape(-1)
+        if h.numel() and (int(h.min()) < 0 or int(h.max()) >= bsz):
+            raise ValueError(f"{name} outside [0, {bsz})")
+        host.append(h)
+        rows.append(h.to(device=device, dtype=torch.int32))
+    if rows[0].numel() != rows[1].numel():
+        raise ValueError("src_rows and dst_rows differ in length")
+    if len(host) == 2:
+        if host[1].unique().numel() != host[1].numel():
+            raise ValueError("dst_rows must be distinct")
+        if bool(torch.isin(host[1], host[0]).any()):
+            raise ValueError("a destination row is also a source row")
+    _on(device, "pagedattn_share_pages", ptr(block_tables), _row_stride(block_tables),
+        block_tables.shape[1], ptr(kv_lens), bsz, ptr(rows[0]), ptr(rows[1]), rows[0].numel(),
+        ptr(ref_counts), ref_counts.numel(), ptr(error_flag))
+
+
+def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, ref_counts: torch.Tensor,
+                  kv_scales: torch.Tensor | None = None,
+                  error_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """The n pages that are held move to ids [0, n) of the pool, in every layer:
+    those there already stay, the k-th held page at or past n goes to the k-th
+    free one below.  ref_counts, the entries of block_tables (and kv_scales) follow
+    in place.  Returns remap [num_pages] int32: each page's new id, -1 for free
+    ones, for tables kept elsewhere (a prefix cache).  error_flag counts entries
+    that name a page outside the pool or a free one; they stay as they are."""
+    n_layers, num_pages, hkv, d, scales = _whole_pool(kv_pool, kv_scales)
+    device = _page_tables(block_tables, ref_counts, num_pages, error_flag, 1)
+    if kv_pool.device != device:
+        raise ValueError("kv_pool and block_tables must be on one device")
+    remap = torch.empty(num_pages, dtype=torch.int32, device=device)
+    scratch = _page_scratch(device, num_pages, block_tables)
+    _on(device, "pagedattn_compact_pages", ptr(kv_pool), dtype_code(kv_pool.dtype), n_layers,
+        num_pages, hkv, d, PAGE_SIZE, ptr(scales), ptr(block_tables), _row_stride(block_tables),
+        block_tables.shape[1], block_tables.shape[0], ptr(ref_counts), ptr(remap),
+        ptr(error_flag), ptr(scratch), scratch.numel())
+    return remap
 
 
 def fork_pages(kv_pool: torch.Tensor, src_pages, dst_pages, valid_tokens=None,
