@@ -158,41 +158,39 @@ struct HalfRegs {
   float sc;  // lane j < 4 holds the scale of the tile's page j
 };
 
+// Page j of tile `tile`; windowed tiles hold the pages that window_page lists.
+template <bool WINDOW>
+__device__ __forceinline__ int tile_page(const WindowTiles& wt, int tile, int j) {
+  if constexpr (WINDOW) return window_page(wt, tile * 4 + j);
+  else return tile * 4 + j;
+}
+
 // Page ids of tile `tile` as a vector load: lane j < 4 gets the id of the
 // tile's page j (-1 past the sequence).  Issued a tile ahead of the K/V
 // loads that use it, it is waited on with the in-order vector counter, so
 // no K/V load ever waits for a page-id fetch.
+template <bool WINDOW>
 __device__ __forceinline__ int fetch_page_ids(const PrefillParams& p,
                                               int ind_lo, int npages,
-                                              int tile, int lane) {
-  const int pg = tile * 4 + lane;
+                                              int tile, int lane, const WindowTiles& wt) {
+  const int pg = tile_page<WINDOW>(wt, tile, lane);
   int id = -1;
   if (lane < 4 && pg < npages && ind_lo >= 0 && ind_lo + pg < p.num_indices)
     id = p.kv_indices[ind_lo + pg];
   return id;
 }
-// Windowed tiles: pages [dead_lo, dead_hi) count as absent.
-template <bool WINDOW>
-__device__ __forceinline__ int fetch_seen_ids(const PrefillParams& p, int ind_lo, int npages,
-                                              int tile, int lane, int dead_lo, int dead_hi) {
-  const int id = fetch_page_ids(p, ind_lo, npages, tile, lane);
-  if constexpr (WINDOW) {
-    const int pg = tile * 4 + lane;
-    if (pg >= dead_lo && pg < dead_hi) return -1;
-  }
-  return id;
-}
+
 
 // Buffer resource of the K (V = false) or V block of tile page j, sized to
 // its valid tokens: absent pages and slots past last_page_len read as zero.
-template <int D, bool BF16, bool FP8, int RB, bool V>
+template <int D, bool BF16, bool FP8, int RB, bool V, bool WINDOW>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(
     const PrefillParams& p, int h, int pid, int npages, int last, int tile,
-    int j) {
+    int j, const WindowTiles& wt) {
   using C = PrefillCfg<D, BF16, FP8, RB>;
   int id = __builtin_amdgcn_readlane(pid, j);
   if (id >= p.num_pages) id = -1;
-  const int pg = tile * 4 + j;
+  const int pg = tile_page<WINDOW>(wt, tile, j);
   const int ntok = id < 0 ? 0 : (pg == npages - 1 ? last : kPage);
   const uint8_t* base =
       p.cache + (((int64_t)(id < 0 ? 0 : id) * 2 + (V ? 1 : 0)) * p.hkv + h) *
@@ -204,11 +202,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(
 // of NW waves.  Wave w's k-th load fills the 1 KiB block NW k + w of the tile
 // (lane i -> bytes [16 i, 16 i + 16) of the block), so each lane fetches the
 // global chunk that the swizzle puts at its position.
-template <int D, bool BF16, bool FP8, int RB, bool V, int NW>
+template <int D, bool BF16, bool FP8, int RB, bool V, int NW, bool WINDOW>
 __device__ __forceinline__ void dma_half(const PrefillParams& p, int h,
                                          int pid, int npages, int last,
                                          int tile, uint8_t* lds, int wave,
-                                         int lane) {
+                                         int lane, const WindowTiles& wt) {
   using C = PrefillCfg<D, BF16, FP8, RB>;
   constexpr int RPB = 1024 / C::ROWB;   // rows per 1 KiB block
   constexpr int CPR = C::ROWB / 16;     // chunks per row
@@ -219,7 +217,7 @@ __device__ __forceinline__ void dma_half(const PrefillParams& p, int h,
     const int row0 = blk * RPB;
     const int j = uniform(row0 / kPage);  // page of the block within the tile
     const __amdgpu_buffer_rsrc_t r =
-        page_rsrc<D, BF16, FP8, RB, V>(p, h, pid, npages, last, tile, j);
+        page_rsrc<D, BF16, FP8, RB, V, WINDOW>(p, h, pid, npages, last, tile, j, wt);
     const int row = row0 + lane / CPR;
     const int c = (lane % CPR) ^ swz<D>(row);
     const uint32_t off = (uint32_t)((row % kPage) * C::ROWB + c * 16);
@@ -231,11 +229,11 @@ __device__ __forceinline__ void dma_half(const PrefillParams& p, int h,
 
 // e4m3 pools: register loads of one half of a K/V tile (16 elements per
 // lane and load at D = 128, 8 at D = 64) plus the four page scales.
-template <int D, bool BF16, bool FP8, int RB, bool V>
+template <int D, bool BF16, bool FP8, int RB, bool V, bool WINDOW>
 __device__ __forceinline__ void load_half(HalfRegs<D, BF16, FP8, RB>& hr,
                                           const PrefillParams& p, int h,
                                           int pid, int npages, int last,
-                                          int tile, int wave, int lane) {
+                                          int tile, int wave, int lane, const WindowTiles& wt) {
   using C = PrefillCfg<D, BF16, FP8, RB>;
   using H = HalfRegs<D, BF16, FP8, RB>;
   constexpr int E = H::WIDE ? 16 : 8;  // elements per lane and load
@@ -247,7 +245,7 @@ __device__ __forceinline__ void load_half(HalfRegs<D, BF16, FP8, RB>& hr,
     // the 64 pieces of a wave lie in one page of the tile
     const int j = uniform((64 * wave + C::THREADS * k) / (D / E) / kPage);
     const __amdgpu_buffer_rsrc_t r =
-        page_rsrc<D, BF16, FP8, RB, V>(p, h, pid, npages, last, tile, j);
+        page_rsrc<D, BF16, FP8, RB, V, WINDOW>(p, h, pid, npages, last, tile, j, wt);
     if constexpr (H::WIDE) {
       hr.x[k] = buf_load16(r, (uint32_t)((tok % kPage) * D + d0));
     } else {
@@ -294,7 +292,7 @@ __device__ __forceinline__ float lane_value(float v, int i) {
 constexpr float kRescaleSlack = 8.f;
 
 // One row of a windowed tile, element by element: what prefill_kernel computes
-// for the tokens of KV tiles [t_lo, t_hi) that the row at position `pos` sees,
+// for the tokens of the walk's tiles [t_lo, t_hi) that the row at position `pos` sees,
 // by all 64 lanes of a wave (lane -> token, then lane -> d).  Called for rows
 // that came out not finite only: a tile's V rows are multiplied for every row
 // of the tile, by a weight of 0 where a row does not see the token, and 0 times an
@@ -315,12 +313,11 @@ __device__ __forceinline__ void window_row(const PrefillParams& p, int h, int in
     else return h2f<BF16>(*reinterpret_cast<const uint16_t*>(x));
   };
   for (int t = t_lo; t < t_hi; ++t) {
-    const int kt = t < wt.sink_tiles ? t : t - wt.sink_tiles + wt.first;
-    const int tok = kt * kPrefillKvTile + lane;
+    const int pg = window_page(wt, 4 * t + lane / kPage);
+    const int tok = pg * kPage + lane % kPage;
     const bool seen = tok < kv_len && tok <= lim &&
                       ((int64_t)tok >= (int64_t)pos - p.window_left || tok < p.sinks);
     int page = -1;
-    const int pg = tok / kPage;
     if (seen && pg < npages && ind_lo >= 0 && ind_lo + pg < p.num_indices)
       page = p.kv_indices[ind_lo + pg];
     if (page >= p.num_pages) page = -1;
@@ -370,7 +367,8 @@ __device__ __forceinline__ void window_row(const PrefillParams& p, int h, int in
 }
 
 template <int D, bool BF16, bool FP8, int RB, bool SPLIT, bool WINDOW>
-__global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillParams p) {
+__global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 ? 4 : 1)
+    prefill_kernel(PrefillParams p) {
   using C = PrefillCfg<D, BF16, FP8, RB>;
   constexpr int BN = C::BN;
   // Two stages, each a K tile then a V tile.  Tile t lives in stage t & 1;
@@ -420,21 +418,10 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       p.causal ? min(kv_len, max(0, diag + q_hi)) : kv_len;
   const int clean_end =
       p.causal ? min(kv_len, max(0, diag + q_lo + 1)) : kv_len;
-  // a windowed tile walks the KV tiles that some row of it sees; tile t of the
-  // walk is KV tile kv_tile(t)
+  // a windowed tile walks the KV pages that some row of it sees (window_tiles)
   WindowTiles wt{0, 0, 0};
   if constexpr (WINDOW)
     wt = window_tiles(kv_end, (int64_t)diag + q_lo, p.window_left, p.sinks);
-  auto kv_tile = [&](int t) {
-    if constexpr (WINDOW) return t < wt.sink_tiles ? t : t - wt.sink_tiles + wt.first;
-    else return t;
-  };
-  // pages whose tokens no row of the tile sees are not read: [dead_lo, dead_hi)
-  int dead_lo = 0, dead_hi = 0;
-  if constexpr (WINDOW) {
-    dead_lo = (int)(((int64_t)p.sinks + kPage - 1) / kPage);
-    dead_hi = max(0, diag + q_lo - p.window_left) / kPage;
-  }
   const int n_tiles = WINDOW ? wt.total : (kv_end + BN - 1) / BN;
   // the KV tiles [t_lo, t_hi) of this workgroup: all of them, or piece k of n
   int t_lo = 0, t_hi = n_tiles, slot = -1;
@@ -520,19 +507,22 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
                        8 * (L & 1);
 
     auto fetch_ids = [&](int t) {
-      return fetch_seen_ids<WINDOW>(p, ind_lo, npages, kv_tile(t), lane, dead_lo, dead_hi);
+      return fetch_page_ids<WINDOW>(p, ind_lo, npages, t, lane, wt);
     };
     HalfRegs<D, BF16, FP8, RB> kr, vr;  // e4m3 staging only
     float ksc_l = 0.f, vsc_l = 0.f;     // e4m3 scales of the computed tile
     int pid = fetch_ids(t_lo);
     if (t_lo < t_hi) {
       if constexpr (FP8) {
-        load_half<D, BF16, FP8, RB, false>(kr, p, h, pid, npages, last, kv_tile(t_lo), wave, lane);
-        load_half<D, BF16, FP8, RB, true>(vr, p, h, pid, npages, last, kv_tile(t_lo), wave, lane);
+        load_half<D, BF16, FP8, RB, false, WINDOW>(kr, p, h, pid, npages, last, t_lo, wave, lane,
+                                                   wt);
+        load_half<D, BF16, FP8, RB, true, WINDOW>(vr, p, h, pid, npages, last, t_lo, wave, lane,
+                                                  wt);
       } else {
-        dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid, npages, last, kv_tile(t_lo), st0, wave, lane);
-        dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid, npages, last, kv_tile(t_lo), st0 + C::TILEB,
-                                             wave, lane);
+        dma_half<D, BF16, FP8, RB, false, NW, WINDOW>(p, h, pid, npages, last, t_lo, st0, wave,
+                                                      lane, wt);
+        dma_half<D, BF16, FP8, RB, true, NW, WINDOW>(p, h, pid, npages, last, t_lo,
+                                                     st0 + C::TILEB, wave, lane, wt);
       }
     }
     int pid_next = fetch_ids(t_lo + 1);
@@ -556,13 +546,14 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
         }
         if (mt == 0) {
           if constexpr (FP8)
-            load_half<D, BF16, FP8, RB, false>(kr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
+            load_half<D, BF16, FP8, RB, false, WINDOW>(kr, p, h, pid_ld, npages, last, t + 1,
+                                                       wave, lane, wt);
         }
       }
 
       // ---- online softmax in log2 units; lane holds 32 of the tile's 64
       // tokens of its row (token 32 mt + 8 (i/4) + 4 half + i%4 in register i)
-      const int tok0 = kv_tile(t) * BN;
+      const int tok0 = t * BN;
       float ksc[4], vsc[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -571,23 +562,31 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        if constexpr (MASK) {
+        if constexpr (MASK && !WINDOW) {
           const int rel = lim[rb] - tok0 - 4 * half;  // visible iff offset <= rel
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (32 * mt + 8 * (i >> 2) + (i & 3) > rel) s[rb][mt][i] = -INFINITY;
-          if constexpr (WINDOW) {
-            const int rel_lo = wlo[rb] - tok0 - 4 * half;  // and offset >= rel_lo, or a sink
-            const int rel_sink = p.sinks - tok0 - 4 * half;
+        }
+        if constexpr (MASK && WINDOW) {
+          // page by page: visible iff offset <= rel, and >= rel_lo or < rel_sink
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+          for (int pg = 0; pg < 4; ++pg) {
+            const int at = kPage * window_page(wt, 4 * t + pg) + 4 * half;
+            const int rel = lim[rb] - at;
+            const int rel_lo = wlo[rb] - at;
+            const int rel_sink = p.sinks - at;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int at = 32 * mt + 8 * (i >> 2) + (i & 3);
-                if (at < rel_lo && at >= rel_sink) s[rb][mt][i] = -INFINITY;
-              }
+            for (int i = 0; i < 8; ++i) {
+              const int off = 8 * (i >> 2) + (i & 3);
+              // without branches: 122 VGPRs at D = 64, where more than 128 would
+              // cost the CU's second workgroup (160 with them)
+              const bool hidden = (off > rel) | ((off < rel_lo) & (off >= rel_sink));
+              const float x = s[rb][pg >> 1][8 * (pg & 1) + i];
+              s[rb][pg >> 1][8 * (pg & 1) + i] = hidden ? -INFINITY : x;
+            }
           }
         }
         // e4m3: the page scale (> 0; FLT_MIN stands in for an empty page,
@@ -642,7 +641,8 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       for (int st = 0; st < 4; ++st) {
         if (st == 1) {
           if constexpr (FP8)
-            load_half<D, BF16, FP8, RB, true>(vr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
+            load_half<D, BF16, FP8, RB, true, WINDOW>(vr, p, h, pid_ld, npages, last, t + 1, wave,
+                                                      lane, wt);
         }
         u32x4 pb[RB];
 #pragma unroll
@@ -694,9 +694,10 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
       if constexpr (!FP8) {
         // tile t + 1 straight into the other stage, K and V, a whole tile
         // ahead of the barrier that waits for it
-        dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1), nxt, wave, lane);
-        dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1), nxt + C::TILEB,
-                                             wave, lane);
+        dma_half<D, BF16, FP8, RB, false, NW, WINDOW>(p, h, pid_ld, npages, last, t + 1, nxt,
+                                                      wave, lane, wt);
+        dma_half<D, BF16, FP8, RB, true, NW, WINDOW>(p, h, pid_ld, npages, last, t + 1,
+                                                     nxt + C::TILEB, wave, lane, wt);
       }
       // paired tiles: a wave with no row of the tile only loads
       if (!decltype(pair_tag)::value || wave_rows) compute(mask_tag, t, cur, pid_ld);
@@ -711,11 +712,11 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
     int n_edge = t_lo, n_clean = 0;
     if constexpr (WINDOW) {
       const int last_lo = diag + q_hi - 1 - p.window_left;
-      if (last_lo > p.sinks)
-        n_edge = max(t_lo, min(t_hi, wt.sink_tiles + max(0, (last_lo + BN - 1) / BN - wt.first)));
-      n_clean = min(t_hi, max(n_edge, last_lo > p.sinks
-                                          ? wt.sink_tiles + max(0, clean_end / BN - wt.first)
-                                          : min(clean_end / BN, n_tiles)));
+      if (last_lo > p.sinks) {
+        const int pages = max(wt.sink_pages, (last_lo + kPage - 1) / kPage - wt.shift);
+        n_edge = max(t_lo, min(t_hi, (pages + 3) / 4));
+      }
+      n_clean = min(t_hi, max(n_edge, (clean_end / kPage - wt.shift) / 4));
     } else {
       n_clean = min(t_hi, SPLIT ? max(t_lo, clean_end / BN) : clean_end / BN);
     }
@@ -751,13 +752,15 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, 1) prefill_kernel(PrefillP
         pid_next = fetch_ids(t + 2);
         const int pid_ld = t + 1 < t_hi ? pid : -1;
         if constexpr (FP8) {
-          load_half<D, BF16, FP8, RB, false>(kr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
-          load_half<D, BF16, FP8, RB, true>(vr, p, h, pid_ld, npages, last, kv_tile(t + 1), wave, lane);
+          load_half<D, BF16, FP8, RB, false, WINDOW>(kr, p, h, pid_ld, npages, last, t + 1, wave,
+                                                     lane, wt);
+          load_half<D, BF16, FP8, RB, true, WINDOW>(vr, p, h, pid_ld, npages, last, t + 1, wave,
+                                                    lane, wt);
         } else {
-          dma_half<D, BF16, FP8, RB, false, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1), nxt, wave,
-                                                lane);
-          dma_half<D, BF16, FP8, RB, true, NW>(p, h, pid_ld, npages, last, kv_tile(t + 1),
-                                               nxt + C::TILEB, wave, lane);
+          dma_half<D, BF16, FP8, RB, false, NW, WINDOW>(p, h, pid_ld, npages, last, t + 1, nxt,
+                                                        wave, lane, wt);
+          dma_half<D, BF16, FP8, RB, true, NW, WINDOW>(p, h, pid_ld, npages, last, t + 1,
+                                                       nxt + C::TILEB, wave, lane, wt);
         }
       }
     }
