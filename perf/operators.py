@@ -41,12 +41,14 @@ DEV = "cuda"
 I32 = torch.int32
 
 
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       "llm-inference-runtime_amd")
+
+
 def _kernels():
     """The framework's package."""
-    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                        "llm-inference-runtime_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if PACKAGE not in sys.path:
+        sys.path.insert(0, PACKAGE)
     import pagedattn
 
     return pagedattn
