@@ -15,6 +15,8 @@
 // returned as an int for the caller to raise.
 #include <Python.h>
 
+#include <cmath>
+
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/Allocator.h>
@@ -36,6 +38,7 @@ struct Entries {
   decltype(&pagedattn_append_paged_kv_cache) append;
   decltype(&pagedattn_rope_append_paged_kv_cache) rope_append;
   decltype(&pagedattn_append_paged_kv_cache_e4m3_amax) append_amax;
+  decltype(&pagedattn_multi_axis_rope_append_paged_kv_cache) axes_append;
 };
 Entries g_entry;
 PyObject* g_raw_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
@@ -414,6 +417,66 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// axes_append(key, value, batch_indices, positions, pool, indices, indptr, scales,
+//             flag, q, rope_scale, rope_theta, axis_positions, sections, cyclic,
+//             rotary_dim, interleave)
+PyObject* axes_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 17)) return nullptr;
+  AppendArgs x;
+  if (!x.get(a)) return general();
+  const at::Tensor* q = rows(a[9], -1, x.pool.d);
+  const at::Tensor* axes = plain(a[12]);
+  if (!q || q->size(0) != x.nnz || q->scalar_type() != x.k->scalar_type() || !axes ||
+      axes->dim() != 2 || axes->size(1) != x.nnz || axes->scalar_type() != at::kInt ||
+      axes->stride(1) != 1 || axes->stride(0) < x.nnz || !PyTuple_CheckExact(a[13]) ||
+      PyTuple_GET_SIZE(a[13]) != axes->size(0) || axes->size(0) < 1 || axes->size(0) > 4 ||
+      !PyFloat_CheckExact(a[10]) || !PyFloat_CheckExact(a[11]) || !PyBool_Check(a[14]) ||
+      !PyBool_Check(a[16]))
+    return general();
+  const at::Device dev = x.pool.device;
+  if (q->device() != dev || x.k->device() != dev || x.v->device() != dev || axes->device() != dev)
+    return general();
+  const double rope_scale = PyFloat_AS_DOUBLE(a[10]), rope_theta = PyFloat_AS_DOUBLE(a[11]);
+  int32_t share[4] = {0, 0, 0, 0};
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[13]); ++i) {
+    PyObject* o = PyTuple_GET_ITEM(a[13], i);
+    if (!PyLong_CheckExact(o)) return general();
+    int over = 0;
+    const long v = PyLong_AsLongAndOverflow(o, &over);
+    if (over || v < 0 || v > INT32_MAX) return general();
+    share[i] = (int32_t)v;
+  }
+  long rotary = 0;
+  if (a[15] != Py_None) {
+    int over = 0;
+    if (!PyLong_CheckExact(a[15])) return general();
+    rotary = PyLong_AsLongAndOverflow(a[15], &over);
+    if (over || rotary < 0 || rotary > INT32_MAX) return general();
+  }
+  // what the general path refuses is left to it
+  if (!(rope_scale > 0) || !(rope_theta > 0) || !std::isfinite(rope_scale) ||
+      !std::isfinite(rope_theta))
+    return general();
+  if (!raw_stream(dev, &x.stream)) return nullptr;
+  void *qp = q->data_ptr(), *kp = x.k->data_ptr(), *pp = x.pool.ptr();
+  const void* vp = x.v->data_ptr();
+  const auto* ap = static_cast<const int32_t*>(axes->data_ptr());
+  const int32_t n_axes = (int32_t)axes->size(0);
+  const bool cyclic = a[14] == Py_True, interleave = a[16] == Py_True;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_entry.axes_append(
+      qp, q->stride(0), q->stride(1), (int32_t)q->size(1), kp, vp, x.k->stride(0), x.k->stride(1),
+      x.v->stride(0), x.v->stride(1), code16(*q), ap, axes->stride(0), n_axes, share, cyclic, x.bi,
+      x.pos, (int32_t)x.nnz, (int32_t)rotary, interleave, (float)rope_scale, (float)rope_theta, pp,
+      x.pool.code, x.scales, (int32_t)x.pool.pages, x.ind, (int32_t)x.n_ind, x.indptr,
+      (int32_t)x.n_ptr - 1, (int32_t)x.pool.hkv, (int32_t)x.pool.d, kPageSize, x.flag, x.stream);
+  Py_END_ALLOW_THREADS
+  return done(rc);
+  END_HANDLE_TH_ERRORS
+}
+
 // append_amax(key, value, batch_indices, positions, pool, indices, indptr, scales, flag)
 PyObject* append_amax(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -456,6 +519,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       reinterpret_cast<decltype(e.rope_append)>(at("pagedattn_rope_append_paged_kv_cache"));
   e.append_amax = reinterpret_cast<decltype(e.append_amax)>(
       at("pagedattn_append_paged_kv_cache_e4m3_amax"));
+  e.axes_append = reinterpret_cast<decltype(e.axes_append)>(
+      at("pagedattn_multi_axis_rope_append_paged_kv_cache"));
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: missing entry point");
     return nullptr;
@@ -474,6 +539,7 @@ PyMethodDef kMethods[] = {
     {"append", FAST(append), nullptr},
     {"rope_append", FAST(rope_append), nullptr},
     {"append_amax", FAST(append_amax), nullptr},
+    {"axes_append", FAST(axes_append), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, kMethods};

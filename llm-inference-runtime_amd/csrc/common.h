@@ -22,7 +22,7 @@ int check_launch(const char* what);
 // CU count of the current device, cached per device.
 int device_cu_count();
 
-inline bool aligned16(const void* p) {
+inline __host__ __device__ bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
 

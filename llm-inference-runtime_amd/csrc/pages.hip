@@ -29,7 +29,19 @@ constexpr int kPagesPerThread = kPagesPerBlock / kPageThreads;
 __device__ __forceinline__ uint32_t live_bits(const int32_t* refs, int64_t p0, int num_pages,
                                               bool past) {
   uint32_t m = 0;
+  if (p0 + kPagesPerThread <= num_pages && aligned16(refs)) {
+    // whole 16-byte loads (p0 is a multiple of 16 pages)
+    int4 v[kPagesPerThread / 4];
 #pragma unroll
+    for (int i = 0; i < kPagesPerThread / 4; ++i)
+      v[i] = reinterpret_cast<const int4*>(refs + p0)[i];
+#pragma unroll
+    for (int i = 0; i < kPagesPerThread / 4; ++i)
+      m |= ((v[i].x != 0 ? 1u : 0u) | (v[i].y != 0 ? 2u : 0u) | (v[i].z != 0 ? 4u : 0u) |
+            (v[i].w != 0 ? 8u : 0u))
+           << (4 * i);
+    return m;
+  }
   for (int i = 0; i < kPagesPerThread; ++i) {
     const bool in = p0 + i < num_pages;
     if (in ? refs[p0 + i] != 0 : past) m |= 1u << i;
@@ -173,13 +185,14 @@ __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs 
     }
     return;
   }
+  // the block's pages are on their way while the counts are summed
+  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
+  uint32_t open = ~live_bits(a.refs, p0, a.num_pages, true) & ((1u << kPagesPerThread) - 1);
   int wanted = 0;
   for (int b = (int)threadIdx.x; b < a.batch; b += kPageThreads) wanted += a.need[b] & ~kForkBit;
   wanted = block_sum(wanted, red);
   const int before = array_sum(a.free_cnt, (int)blockIdx.x, red);
   if (before >= wanted) return;  // uniform
-  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-  uint32_t open = ~live_bits(a.refs, p0, a.num_pages, true) & ((1u << kPagesPerThread) - 1);
   int total;
   __syncthreads();
   int rank = before + block_excl_scan<kPageThreads>(__builtin_popcount(open), &total, red);
@@ -395,21 +408,30 @@ __global__ void __launch_bounds__(kPageThreads) compact_count_kernel(CompactArgs
 
 __global__ void __launch_bounds__(kPageThreads) compact_rank_kernel(CompactArgs a) {
   __shared__ int red[kPageThreads / kWave];
-  const int n_live = array_sum(a.live_cnt, a.n_blocks, red);
+  // this block's pages are on their way while the counts are summed
+  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
+  const uint32_t live = live_bits(a.refs, p0, a.num_pages, false);
+  int all = 0, mine = 0;
+  for (int i = (int)threadIdx.x; i < a.n_blocks; i += kPageThreads) {
+    const int n = a.live_cnt[i];
+    all += n;
+    mine += i < (int)blockIdx.x ? n : 0;
+  }
+  const int n_live = block_sum(all, red);
+  const int before_blk = block_sum(mine, red);
   // live pages below n_live, which stay
   const int line_blk = min(n_live / kPagesPerBlock, a.n_blocks - 1);
   const int64_t l0 = (int64_t)line_blk * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
   uint32_t below = live_bits(a.refs, l0, a.num_pages, false);
   const int64_t inside = n_live - l0;  // of this thread's pages, those below the line
   below &= inside >= kPagesPerThread ? ~0u : inside > 0 ? (1u << (int)inside) - 1 : 0u;
-  const int stay = array_sum(a.live_cnt, line_blk, red) + block_sum(__builtin_popcount(below), red);
-  const int before_blk = array_sum(a.live_cnt, (int)blockIdx.x, red);
+  int under = __builtin_popcount(below);
+  for (int i = (int)threadIdx.x; i < line_blk; i += kPageThreads) under += a.live_cnt[i];
+  const int stay = block_sum(under, red);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     *a.n_live = n_live;
     *a.n_moves = n_live - stay;
   }
-  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-  const uint32_t live = live_bits(a.refs, p0, a.num_pages, false);
   int total;
   __syncthreads();
   int before = before_blk +

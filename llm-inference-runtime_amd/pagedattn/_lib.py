@@ -257,6 +257,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_of(device: torch.device) -> int:
     """hipStream_t of torch's current stream on `device` (as an int)."""
+    if device.type == "cuda" and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)  # no Stream object
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -311,7 +311,7 @@ def rope_append_paged_kv_cache(q: torch.Tensor, append_key: torch.Tensor,
 def _on(device: torch.device, name: str, *args) -> None:
     """Entry point `name` on `device` and its current stream, whichever device
     is current."""
-    if device.index in (None, torch.cuda.current_device()):
+    if device.index == torch._C._cuda_getDevice():
         call(name, *args, _stream(device))
     else:
         with torch.cuda.device(device):
@@ -383,6 +383,12 @@ def multi_axis_rope_append_paged_kv_cache(
     by append_paged_kv_cache(...) in one launch, with the results of the two.
     `positions` are the tokens' places in the cache, which the axis positions of
     images and of text after them differ from."""
+    if kv_layout == "HND" and _native(
+            "axes_append", "pagedattn_multi_axis_rope_append_paged_kv_cache", append_key,
+            append_value, batch_indices, positions, paged_kv_cache, kv_indices, kv_indptr,
+            kv_scales, error_flag, q, rope_scale, rope_theta, axis_positions, sections, cyclic,
+            rotary_dim, interleave) is None:
+        return
     num_pages, hkv, d = _check_pool(paged_kv_cache, None, None, kv_layout)
     _check_rows(q, "q", None, d)
     _check_rows(append_key, "append_key", hkv, d)
@@ -1007,9 +1013,9 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         n, device = self._bsz, self._indptr.device
         per_seq = -(-sinks // PAGE_SIZE) + left // PAGE_SIZE + 2
         room = min(self._indices.numel(), n * per_seq)
-        self._seen_indptr = torch.zeros(n + 1, dtype=torch.int32, device=device)
-        self._seen_indices = torch.empty(max(room, 1), dtype=torch.int32, device=device)[:room]
-        self._holes = torch.empty((max(n, 1), 4), dtype=torch.int32, device=device)[:n]
+        buf = torch.empty(5 * n + 1 + max(room, 1), dtype=torch.int32, device=device)
+        self._holes, self._seen_indptr, self._seen_indices = buf.split(
+            [4 * n, n + 1, max(room, 1)])
         if lists_now:
             self._make_lists()
         self._planned = True

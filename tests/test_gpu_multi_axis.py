@@ -90,7 +90,21 @@ def test_equal_positions_are_the_one_position_call(gpu, rotary, interleave):
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("interleave", [False, True])
 @pytest.mark.parametrize("chunks", [[1] * 9, [40, 1, 130, 17]])
-def test_append_is_the_two_calls(gpu, d, rotary, sections, cyclic, fp8, interleave, chunks):
+@pytest.mark.parametrize("native", [True, False])
+def test_append_is_the_two_calls(gpu, d, rotary, sections, cyclic, fp8, interleave, chunks,
+                                 native, monkeypatch):
+    """By the extension's call and by the general path."""
+    if native:
+        real = pagedattn.ops._native
+
+        def taken(fn, *args):
+            r = real(fn, *args)
+            assert r is not NotImplemented, fn
+            return r
+
+        monkeypatch.setattr(pagedattn.ops, "_native", taken)
+    else:
+        monkeypatch.setattr(pagedattn.ops, "_native", lambda *a: NotImplemented)
     dtype, hq, hkv, n = torch.bfloat16, 8, 2, sum(chunks)
     rng = np.random.default_rng(n)
     g = torch.Generator(device=gpu)
