@@ -20,6 +20,10 @@ Deliberate differences from the reference:
   the scales of the pages it writes a running amax
   (``append_paged_kv_cache_e4m3_amax``); ``"fixed"`` encodes with the scales
   as given (pools quantised ahead of time).
+* Attention may be windowed (``FlashInferState.window_left`` and
+  ``num_sink_tokens``): every token sees the window_left tokens before it and
+  the sequence's first num_sink_tokens, prefill and decode alike.  Pages that
+  fell out of the window may be freed (-1 in the step's page lists).
 """
 
 from __future__ import annotations
@@ -46,6 +50,8 @@ class FlashInferState:
     kv_pool: torch.Tensor | None = None
     kv_scales: torch.Tensor | None = None  # e4m3 pools only: [L, P, 2, Hkv]
     kv_scale_policy: str = "running"  # e4m3 pools: "running" amax or "fixed" scales
+    window_left: int = -1  # tokens seen before a token (-1: all)
+    num_sink_tokens: int = 0  # first tokens that stay visible behind a window
 
     kv_indices: torch.Tensor | None = None
     kv_indptr: torch.Tensor | None = None
@@ -75,9 +81,11 @@ WORKSPACE_BYTES = 128 * 1024 * 1024
 
 def init_flashinfer_state(*, kv_pool: torch.Tensor, page_size: int, device,
                           kv_scales: torch.Tensor | None = None,
-                          kv_scale_policy: str = "running") -> None:
+                          kv_scale_policy: str = "running", window_left: int = -1,
+                          num_sink_tokens: int = 0) -> None:
     """Store the pool, allocate the 128 MiB workspace and the two wrappers
     (src/models/llama.py:39-67)."""
+    window_left, num_sink_tokens = ops._window(window_left, num_sink_tokens)
     if page_size != ops.PAGE_SIZE:
         raise NotImplementedError(f"page_size {page_size} (only 16 is implemented)")
     if kv_scale_policy not in ("running", "fixed"):
@@ -85,6 +93,8 @@ def init_flashinfer_state(*, kv_pool: torch.Tensor, page_size: int, device,
     FlashInferState.kv_pool = kv_pool
     FlashInferState.kv_scales = kv_scales
     FlashInferState.kv_scale_policy = kv_scale_policy
+    FlashInferState.window_left = window_left
+    FlashInferState.num_sink_tokens = num_sink_tokens
     FlashInferState.page_size = page_size
     FlashInferState.dtype = kv_pool.dtype
     ws = torch.zeros(WORKSPACE_BYTES, dtype=torch.uint8, device=device)
@@ -150,6 +160,8 @@ def plan_prefill(*, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor, kv_indices
     pw = cast(ops.BatchPrefillWithPagedKVCacheWrapper, FlashInferState.prefill_wrapper)
     pw.begin_forward(qo_indptr, kv_indptr, kv_indices, kv_last_page_len, num_qo_heads,
                      num_kv_heads, head_dim, FlashInferState.page_size, q_data_type=_q_dtype(),
+                     window_left=FlashInferState.window_left,
+                     num_sink_tokens=FlashInferState.num_sink_tokens,
                      device_plan=max_qo_tokens is not None, max_qo_tokens=max_qo_tokens)
 
 
@@ -180,6 +192,8 @@ def plan_decode(*, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
     dw = cast(ops.BatchDecodeWithPagedKVCacheWrapper, FlashInferState.decode_wrapper)
     dw.begin_forward(kv_indptr, kv_indices, kv_last_page_len, num_qo_heads, num_kv_heads,
                      head_dim, FlashInferState.page_size, q_data_type=_q_dtype(),
+                     window_left=FlashInferState.window_left,
+                     num_sink_tokens=FlashInferState.num_sink_tokens,
                      indptr_host=indptr_h.reshape(kv_indptr.shape),
                      last_page_len_host=last_h.reshape(kv_last_page_len.shape))
     FlashInferState._fused_rows = (

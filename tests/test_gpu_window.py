@@ -7,6 +7,7 @@ to the 16-bit type (half a step u, relative), scores are sums of D products in
 exp(2 s) - 1; fp16 weights below 2^-24 of a row's largest round to multiples
 of 2^-24."""
 
+import copy
 import math
 
 import numpy as np
@@ -14,6 +15,7 @@ import pytest
 import torch
 
 import pagedattn
+from pagedattn import llama as L
 from pagedattn.metadata import decode_metadata, prefill_metadata
 
 from paged_cases import i32, random_tables, require_shared_plans, strided_rows, workspace
@@ -364,3 +366,95 @@ def test_decode_step_replayed_from_a_graph(gpu):
             want = we.run(q, pool, append_key=k, append_value=v, rope=(1.0, 10000.0))
             assert torch.equal(got, want), i
             assert torch.equal(wrote, pool), i
+
+
+def test_forward_takes_the_planned_window_only(gpu):
+    heads, dtype = HEADS[1], torch.bfloat16
+    meta, pool, _, q = make(gpu, [40, 9], [1, 1], heads, dtype, False, 20, 4, seed=1)
+    w = plan_decode(gpu, meta, heads, dtype, 20, 4, "device")
+    assert torch.equal(w.forward(q, pool, window_left=20), w.forward(q, pool))
+    pw = plan_prefill(gpu, meta, heads, dtype, -1, 0, False)
+    for x, left in ((w, 21), (w, 0), (pw, 20)):
+        with pytest.raises(ValueError, match="window"):
+            x.forward(q, pool, window_left=left)
+    for left, sinks in ((-2, 0), (-1, 4), (None, 1), (5, -1), (1 << 31, 0)):
+        for x in (w, pw):
+            args = [i32(meta.kv_indptr, gpu), i32(meta.kv_indices, gpu),
+                    i32(meta.kv_last_page_len, gpu), *heads, 16]
+            if x is pw:
+                args.insert(0, i32(meta.qo_indptr, gpu))
+            with pytest.raises(ValueError):
+                x.plan(*args, window_left=left, num_sink_tokens=sinks)
+
+
+def test_an_empty_batch(gpu):
+    w = pagedattn.BatchDecodeWithPagedKVCacheWrapper(workspace(gpu), "HND")
+    for device_plan in (False, True):
+        w.plan(i32([0], gpu), i32([], gpu), i32([], gpu), 8, 2, 64, 16, window_left=5,
+               num_sink_tokens=2, device_plan=device_plan)
+        out = w.run(torch.zeros((0, 8, 64), dtype=torch.float16, device=gpu),
+                    torch.zeros((3, 2, 2, 16, 64), dtype=torch.float16, device=gpu))
+        assert out.shape == (0, 8, 64)
+
+
+def test_patched_llama_with_a_window(gpu):
+    """The engine's shim, fused and not, against the model under the window's mask in 32 bits on
+    the CPU; pages behind the window are gone by the decode step."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from pagedattn.metadata import decode_metadata, prefill_metadata
+
+    cfg = LlamaConfig(hidden_size=512, intermediate_size=1024, num_attention_heads=8,
+                      num_key_value_heads=2, num_hidden_layers=2, vocab_size=512,
+                      max_position_embeddings=4096, attn_implementation="eager")
+    torch.manual_seed(0)
+    ref = LlamaForCausalLM(cfg).eval()
+    model = copy.deepcopy(ref).to(device=gpu, dtype=torch.bfloat16)
+    L.patch_llama_model(model)
+    window, sinks, lens = 24, 5, [37, 100, 5, 64]
+    rng = np.random.default_rng(0)
+    tokens = torch.as_tensor(rng.integers(0, 512, (len(lens), 128)))
+    tables, num_pages = random_tables(rng, [n + 1 for n in lens], extra_pages=4)
+    got = []
+    try:
+        for L.FUSE in (True, False):
+            pool = torch.zeros((2, num_pages, 2, 2, 16, 64), dtype=torch.bfloat16, device=gpu)
+            L.init_flashinfer_state(kv_pool=pool, page_size=16, device=gpu, window_left=window,
+                                    num_sink_tokens=sinks)
+            meta = prefill_metadata(tables, [0] * len(lens), lens)
+            L.build_batch_indices_positions(i32(meta.qo_indptr, gpu), i32(meta.seq_lens, gpu))
+            shape = dict(num_qo_heads=8, num_kv_heads=2, head_dim=64)
+            L.plan_prefill(qo_indptr=i32(meta.qo_indptr, gpu), kv_indptr=i32(meta.kv_indptr, gpu),
+                           kv_indices=i32(meta.kv_indices, gpu),
+                           kv_last_page_len=i32(meta.kv_last_page_len, gpu), **shape)
+            packed = torch.cat([tokens[b, :n] for b, n in enumerate(lens)])[None].to(gpu)
+            with torch.no_grad():
+                pre = model(input_ids=packed, use_cache=False).logits[0]
+            kept = [[p if s < 1 or s >= (n - window) // 16 else -1 for s, p in enumerate(t)]
+                    for t, n in zip(tables, lens)]
+            meta = decode_metadata(kept, [n + 1 for n in lens])
+            L.FlashInferState.batch_indices = i32(meta.batch_indices, gpu)
+            L.FlashInferState.positions = i32(meta.positions, gpu)
+            L.plan_decode(kv_indptr=i32(meta.kv_indptr, gpu),
+                          kv_indices=i32(meta.kv_indices, gpu),
+                          kv_last_page_len=i32(meta.kv_last_page_len, gpu), **shape)
+            step = torch.stack([tokens[b, n] for b, n in enumerate(lens)])[:, None].to(gpu)
+            with torch.no_grad():
+                dec = model(input_ids=step, use_cache=False).logits[:, 0]
+            assert L.append_error_count() == 0
+            got.append((pre.float().cpu(), dec.float().cpu()))
+    finally:
+        L.FUSE = True
+        L.init_flashinfer_state(kv_pool=pool, page_size=16, device=gpu)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    ends = np.cumsum(lens)
+    for b, n in enumerate(lens):
+        i, j = torch.arange(n + 1)[:, None], torch.arange(n + 1)
+        seen = (j <= i) & ((j >= i - window) | (j < sinks))
+        mask = torch.where(seen, 0.0, torch.finfo(torch.float32).min)[None, None]
+        with torch.no_grad():
+            full = ref(input_ids=tokens[b:b + 1, :n + 1], attention_mask=mask,
+                       use_cache=False).logits[0]
+        # the bound that the shim's tests without a window have for bf16
+        for mine, want in ((got[0][0][ends[b] - n:ends[b]], full[:n]), (got[0][1][b], full[n])):
+            assert float((mine - want).norm() / want.norm()) < 3e-2, b
