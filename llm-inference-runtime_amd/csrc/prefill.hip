@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
       const int qi = q_lo + row / g;
       rvalid[rb] = qi < q_hi;
       lim[rb] = p.causal ? min(diag + qi, kv_len - 1) : kv_len - 1;
-      if constexpr (WINDOW) wlo[rb] = max(0, diag + qi - p.window_left);
+      if constexpr (WINDOW) wlo[rb] = max(0, diag + qi) - min(max(0, diag + qi), p.window_left);
       const uint16_t* qp =
           p.q + (int64_t)(qo_start + (rvalid[rb] ? qi : q_lo)) * p.q_sn +
           (int64_t)(h * g + row % g) * p.q_sh + 8 * half;
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
     // masked too, [t_lo, n_edge), unless no row's window leaves anything out.
     int n_edge = t_lo, n_clean = 0;
     if constexpr (WINDOW) {
-      const int last_lo = diag + q_hi - 1 - p.window_left;
+      const int last_lo = max(0, diag + q_hi - 1) - min(max(0, diag + q_hi - 1), p.window_left);
       if (last_lo > p.sinks) {
         const int pages = max(wt.sink_pages, (last_lo + kPage - 1) / kPage - wt.shift);
         n_edge = max(t_lo, min(t_hi, (pages + 3) / 4));
@@ -777,14 +777,16 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
       const float2 lh = swap_halves32(l[rb]);
       float l_tot = lh.x + lh.y;
       if constexpr (WINDOW) {
-        // rows that are not finite, one by one (window_row)
-        float x = l_tot * 0.f;
+        // rows that are not finite, one by one (window_row); one whose scores hold a
+        // NaN is NaN as it is
+        float x = 0.f;
 #pragma unroll
         for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) x = __builtin_fmaf(o[rb][dt][i], 0.f, x);
         const float2 xh = swap_halves32(x);
-        uint32_t bad = (uint32_t)__builtin_amdgcn_ballot_w64(rvalid[rb] && !(xh.x + xh.y == 0.f));
+        uint32_t bad = (uint32_t)__builtin_amdgcn_ballot_w64(
+            rvalid[rb] && l_tot == l_tot && !(xh.x + xh.y == 0.f));
         while (bad) {
           const int i = __builtin_ctz(bad);
           bad &= bad - 1;

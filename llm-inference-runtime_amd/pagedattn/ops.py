@@ -933,6 +933,7 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
                  paged_kv_indices_buffer: torch.Tensor | None = None,
                  paged_kv_last_page_len_buffer: torch.Tensor | None = None, **kw):
         super().__init__(float_workspace_buffer, kv_layout, use_cuda_graph, **kw)
+        self._list_bufs = {}
         self._graph_bufs = None
         if use_cuda_graph:
             bufs = (paged_kv_indptr_buffer, paged_kv_indices_buffer,
@@ -1013,9 +1014,16 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         n, device = self._bsz, self._indptr.device
         per_seq = -(-sinks // PAGE_SIZE) + left // PAGE_SIZE + 2
         room = min(self._indices.numel(), n * per_seq)
-        buf = torch.empty(5 * n + 1 + max(room, 1), dtype=torch.int32, device=device)
-        self._holes, self._seen_indptr, self._seen_indices = buf.split(
-            [4 * n, n + 1, max(room, 1)])
+        # one buffer for every size class (powers of two), kept as long as the
+        # wrapper: a captured step holds on to those of the plan it was captured with
+        rows, room = (1 << max(x - 1, 0).bit_length() for x in (n, room))
+        buf = self._list_bufs.get((rows, room, device))
+        if buf is None:
+            buf = torch.empty(5 * rows + 1 + room, dtype=torch.int32, device=device)
+            self._list_bufs[rows, room, device] = buf
+        self._holes = buf[:4 * n]
+        self._seen_indptr = buf[4 * rows:4 * rows + n + 1]
+        self._seen_indices = buf[5 * rows + 1:]
         if lists_now:
             self._make_lists()
         self._planned = True
@@ -1105,7 +1113,9 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         of the decode step runs inside the same launch (the engine's decode
         step: batch_indices = arange(B), positions = kv_len - 1).  With
         rope=(rope_scale, rope_theta) as well, q and append_key are rotated
-        (non-interleaved RoPE at `positions`, default kv_len - 1) inside that
+        (non-interleaved RoPE at `positions`, default kv_len - 1; with a window
+        one that lies behind it is skipped and counted, as one outside the
+        sequence's pages is) inside that
         launch too: apply_rope_pos_ids_inplace + append + attention in one
         kernel (q and append_key themselves are left unrotated)."""
         if not self._planned:

@@ -458,3 +458,64 @@ def test_patched_llama_with_a_window(gpu):
         # the bound that the shim's tests without a window have for bf16
         for mine, want in ((got[0][0][ends[b] - n:ends[b]], full[:n]), (got[0][1][b], full[n])):
             assert float((mine - want).norm() / want.norm()) < 3e-2, b
+
+
+def test_replanning_between_replays_leaves_the_captured_step_its_lists(gpu):
+    """A device plan is captured; the wrapper is planned and run for other batches; the replays
+    still give the first batch's results."""
+    heads, dtype, window, sinks = HEADS[0], torch.float16, 60, 17
+    meta, pool, _, q = make(gpu, [200, 90, 300], [1] * 3, heads, dtype, False, window, sinks, 1)
+    w = plan_decode(gpu, meta, heads, dtype, window, sinks, "device")
+    want = w.run(q, pool)
+    out = torch.zeros_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.run(q, pool, out=out)
+    lists = (w._indptr, w._indices, w._last)  # the caller's metadata, still alive
+    for n, left in ((3, 60), (9, 60), (2, 500), (300, 10)):
+        lens = [100 + 3 * i for i in range(n)]
+        m2, p2, _, q2 = make(gpu, lens, [1] * n, heads, dtype, False, left, sinks, 2)
+        w.plan(*(i32(x, gpu) for x in (m2.kv_indptr, m2.kv_indices, m2.kv_last_page_len)), *heads,
+               16, q_data_type=dtype, window_left=left, num_sink_tokens=sinks,
+               device_plan=n != 9)
+        got = w.run(q2, p2)
+        rows = [0, n - 1]
+        check(got, None, reference(m2, p2, None, q2, left, sinks, b_rows=set(rows)), rows)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+    del lists
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_prefill_of_nan_scores_is_nan(gpu, fp8):
+    """A NaN in a K row: every row that sees it is NaN, the others are as if it were not there."""
+    heads, dtype, window, sinks = HEADS[1], torch.bfloat16, 25, 0
+    meta, pool, scales, q = make(gpu, [0], [100], heads, dtype, fp8, window, sinks, seed=8)
+    page = int(meta.kv_indices[2])
+    pool[page, 0, :, 5] = math.nan  # token 37
+    w = plan_prefill(gpu, meta, heads, dtype, window, sinks, False)
+    out, lse = w.run(q, pool, kv_scales=scales, return_lse=True)
+    seen = list(range(37, 37 + window + 1))
+    clear = sorted(set(range(100)) - set(seen))
+    check(out, lse, reference(meta, pool, scales, q, window, sinks, b_rows=set(clear)), clear)
+    assert bool(torch.isnan(out[seen]).all())
+
+
+def test_a_window_of_the_largest_size(gpu):
+    """Rows before the first token (more rows than tokens) and windows up to 2^31 - 1."""
+    heads, dtype, window, sinks = HEADS[0], torch.float16, (1 << 31) - 1, (1 << 31) - 1
+    meta, pool, scales, q = make(gpu, [0], [60], heads, dtype, False, window, 0, seed=1,
+                                 spoil=False)
+    meta.kv_indptr[1:] = 2
+    meta.kv_last_page_len[0] = 5
+    for s in (0, sinks):
+        for device_plan in (False, True):
+            w = plan_prefill(gpu, meta, heads, dtype, window, s, device_plan)
+            check(*w.run(q, pool, return_lse=True),
+                  reference(meta, pool, scales, q, window, s))
+    one, pool, scales, q = make(gpu, [40, 0], [1, 1], heads, dtype, False, window, 0, seed=1)
+    for kind in ("host", "device"):
+        w = plan_decode(gpu, one, heads, dtype, window, sinks, kind)
+        check(*w.run(q, pool, return_lse=True), reference(one, pool, scales, q, window, sinks))
