@@ -8,6 +8,8 @@
 // by one through ctypes, with the shape checks and strides read in Python, took
 // 12-15 us a call where the attention kernels take 5-10 us on the GPU.
 //
+// The page calls of every captured or eager step take the same way.
+//
 // Returns the call's result, or NotImplemented for anything but the plain form
 // (another type or device, a tensor subclass, metadata that needs a conversion,
 // empty rows, and every bad argument): the caller then takes the general path in
@@ -15,6 +17,7 @@
 // returned as an int for the caller to raise.
 #include <Python.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include <ATen/core/Tensor.h>
@@ -39,6 +42,9 @@ struct Entries {
   decltype(&pagedattn_rope_append_paged_kv_cache) rope_append;
   decltype(&pagedattn_append_paged_kv_cache_e4m3_amax) append_amax;
   decltype(&pagedattn_multi_axis_rope_append_paged_kv_cache) axes_append;
+  decltype(&pagedattn_page_scratch_bytes) page_scratch;
+  decltype(&pagedattn_reserve_pages) reserve;
+  decltype(&pagedattn_release_window_pages) release_window;
 };
 Entries g_entry;
 PyObject* g_raw_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
@@ -498,6 +504,112 @@ PyObject* append_amax(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Page tables of a step, with their counts: int32 [batch, max_pages], rows
+// contiguous.
+struct Tables {
+  int32_t *tables = nullptr, *refs = nullptr, *flag = nullptr;
+  const int32_t* lens = nullptr;
+  int64_t batch = 0, width = 0, stride = 0, pages = 0;
+  at::Device device = at::kCPU;
+  // a flat int32 tensor on the tables' device; count < 0: any length
+  bool ints(PyObject* o, int64_t count, int32_t** out, int64_t* numel = nullptr) {
+    const at::Tensor* t = plain(o);
+    if (!t || t->dim() != 1 || t->device() != device || t->scalar_type() != at::kInt ||
+        !t->is_contiguous() || (count >= 0 && t->numel() != count))
+      return false;
+    *out = static_cast<int32_t*>(t->data_ptr());
+    if (numel) *numel = t->numel();
+    return true;
+  }
+  bool get(PyObject* tables_o, PyObject* lens_o, PyObject* refs_o, PyObject* flag_o, int64_t flags) {
+    const at::Tensor* t = plain(tables_o);
+    if (!t || !t->is_cuda() || t->dim() != 2 || t->scalar_type() != at::kInt || t->size(0) < 1 ||
+        t->size(1) < 1 || t->size(0) > INT32_MAX || t->size(1) > INT32_MAX || t->stride(1) != 1 ||
+        (t->size(0) > 1 && t->stride(0) < t->size(1)))
+      return false;
+    device = t->device();
+    batch = t->size(0);
+    width = t->size(1);
+    stride = std::max(t->stride(0), width);
+    tables = static_cast<int32_t*>(t->data_ptr());
+    int32_t* l = nullptr;
+    if (!ints(lens_o, batch, &l) || !ints(refs_o, -1, &refs, &pages) || pages > INT32_MAX)
+      return false;
+    lens = l;
+    if (flag_o == Py_None) return true;
+    const at::Tensor* f = plain(flag_o);
+    return f && f->device() == device && get_flag(flag_o, flags, &flag);
+  }
+};
+
+// reserve(pool, tables, kv_lens, new_lens, ref_counts, scales, flag)
+PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 7)) return nullptr;
+  Tables x;
+  const at::Tensor* pool = plain(a[0]);
+  if (!pool || !x.get(a[1], a[2], a[4], a[6], 2) || pool->device() != x.device ||
+      pool->dim() != 6 || pool->size(2) != 2 || pool->size(4) != kPageSize ||
+      !pool->is_contiguous() || pool->size(1) != x.pages || pool->size(0) > INT32_MAX ||
+      pool->size(3) > INT32_MAX || pool->size(5) > INT32_MAX)
+    return general();
+  const int code = pool->scalar_type() == at::kFloat8_e4m3fn ? PAGEDATTN_E4M3 : code16(*pool);
+  if (code < 0) return general();
+  int32_t* added = nullptr;
+  if (a[3] != Py_None && !x.ints(a[3], x.batch, &added)) return general();
+  float* scales = nullptr;
+  if (code == PAGEDATTN_E4M3) {
+    const at::Tensor* t = plain(a[5]);
+    if (!t || t->device() != x.device || t->scalar_type() != at::kFloat || t->dim() != 4 ||
+        t->size(0) != pool->size(0) || t->size(1) != x.pages || t->size(2) != 2 ||
+        t->size(3) != pool->size(3) || !t->is_contiguous())
+      return general();
+    scales = static_cast<float*>(t->data_ptr());
+  }
+  void* stream;
+  if (!raw_stream(x.device, &stream)) return nullptr;
+  const c10::DeviceGuard guard(x.device);
+  const size_t bytes = g_entry.page_scratch((int32_t)x.pages, (int32_t)x.batch, (int32_t)x.width);
+  const c10::DataPtr scratch =
+      c10::GetAllocator(c10::DeviceType::CUDA)->allocate(std::max<size_t>(bytes, 256));
+  void* pp = pool->data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_entry.reserve(pp, code, (int32_t)pool->size(0), (int32_t)x.pages, (int32_t)pool->size(3),
+                       (int32_t)pool->size(5), kPageSize, scales, x.tables, x.stride,
+                       (int32_t)x.width, x.lens, added, (int32_t)x.batch, x.refs, x.flag,
+                       scratch.get(), bytes, stream);
+  Py_END_ALLOW_THREADS
+  return done(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// release_window(tables, kv_lens, ref_counts, window_left, sinks, flag)
+PyObject* release_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 6)) return nullptr;
+  Tables x;
+  if (!x.get(a[0], a[1], a[2], a[5], 1)) return general();
+  int32_t window[2];
+  for (int i = 0; i < 2; ++i) {
+    int over = 0;
+    if (!PyLong_CheckExact(a[3 + i])) return general();
+    const long v = PyLong_AsLongAndOverflow(a[3 + i], &over);
+    if (over || v < 0 || v > INT32_MAX) return general();
+    window[i] = (int32_t)v;
+  }
+  void* stream;
+  if (!raw_stream(x.device, &stream)) return nullptr;
+  const c10::DeviceGuard guard(x.device);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_entry.release_window(x.tables, x.stride, (int32_t)x.width, x.lens, (int32_t)x.batch,
+                              x.refs, (int32_t)x.pages, window[0], window[1], x.flag, stream);
+  Py_END_ALLOW_THREADS
+  return done(rc);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(raw_stream, {name: address}): the current-stream function and the C
 // entry points, once, before any other call
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -521,6 +633,11 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
       at("pagedattn_append_paged_kv_cache_e4m3_amax"));
   e.axes_append = reinterpret_cast<decltype(e.axes_append)>(
       at("pagedattn_multi_axis_rope_append_paged_kv_cache"));
+  e.page_scratch =
+      reinterpret_cast<decltype(e.page_scratch)>(at("pagedattn_page_scratch_bytes"));
+  e.reserve = reinterpret_cast<decltype(e.reserve)>(at("pagedattn_reserve_pages"));
+  e.release_window =
+      reinterpret_cast<decltype(e.release_window)>(at("pagedattn_release_window_pages"));
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: missing entry point");
     return nullptr;
@@ -540,6 +657,8 @@ PyMethodDef kMethods[] = {
     {"rope_append", FAST(rope_append), nullptr},
     {"append_amax", FAST(append_amax), nullptr},
     {"axes_append", FAST(axes_append), nullptr},
+    {"reserve", FAST(reserve), nullptr},
+    {"release_window", FAST(release_window), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, kMethods};

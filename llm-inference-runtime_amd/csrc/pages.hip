@@ -82,14 +82,14 @@ struct ReserveArgs {
   int32_t* err;
   // scratch: pages wanted by each sequence (kForkBit: one of them for a fork),
   // the sum over those before it, free pages of each block, the pages taken in
-  // order (`cap` at most) and the forks
+  // order, and the forks: the page, the rank of the one that takes its rows, how many
   int32_t* need;
   int32_t* base;
   int32_t* free_cnt;
   int32_t* fresh;
-  int32_t* n_forks;
+  int32_t* n_forks;  // 0 where the pages do not suffice
   int32_t* fork_src;
-  int32_t* fork_dst;
+  int32_t* fork_rank;
   int32_t* fork_rows;
   int32_t* short_of;  // pages missing; nothing is changed then
 };
@@ -130,10 +130,6 @@ __global__ void __launch_bounds__(kPageThreads) reserve_count_kernel(ReserveArgs
     const uint32_t live = live_bits(a.refs, p0, a.num_pages, true);
     const int n = block_sum(kPagesPerThread - __builtin_popcount(live), red);
     if (threadIdx.x == 0) a.free_cnt[blockIdx.x] = n;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      *a.n_forks = 0;
-      *a.short_of = 0;
-    }
     return;
   }
   const int b = ((int)blockIdx.x - a.n_blocks) * (kPageThreads / kWave) +
@@ -163,25 +159,36 @@ __global__ void __launch_bounds__(kPageThreads) reserve_count_kernel(ReserveArgs
 }
 
 // Workgroups [0, n_blocks): the free pages of a block at their ranks, as far as
-// they are wanted.  The last: the sequences' first ranks, and whether the pages
-// suffice.
+// they are wanted.  The last: the sequences' first ranks, the forks, and whether
+// the pages suffice.
 __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs a) {
   __shared__ int red[kPageThreads / kWave];
   if ((int)blockIdx.x == a.n_blocks) {
     const int total_free = array_sum(a.free_cnt, a.n_blocks, red);
-    int run = 0;
+    int run = 0, forks = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
       const int b = b0 + (int)threadIdx.x;
-      const int n = b < a.batch ? a.need[b] & ~kForkBit : 0;
-      int total;
+      const int need = b < a.batch ? a.need[b] : 0;
+      const bool fork = need & kForkBit;
+      int total, total_forks;
       __syncthreads();
-      const int at = block_excl_scan<kPageThreads>(n, &total, red);
-      if (b < a.batch) a.base[b] = run + at;
+      const int at = run + block_excl_scan<kPageThreads>(need & ~kForkBit, &total, red);
+      const int f = forks + block_excl_scan<kPageThreads>(fork ? 1 : 0, &total_forks, red);
+      if (b < a.batch) a.base[b] = at;
+      if (fork) {
+        const RowStep r = row_step(a, b);
+        a.fork_src[f] = a.tables[b * a.stride + r.part];
+        a.fork_rank[f] = at;
+        a.fork_rows[f] = r.rows;
+      }
       run += total;
+      forks += total_forks;
     }
-    if (threadIdx.x == 0 && run > total_free) {
-      *a.short_of = run - total_free;
-      if (a.err) atomicAdd(a.err + 1, run - total_free);
+    if (threadIdx.x == 0) {
+      const int missing = max(run - total_free, 0);
+      *a.short_of = missing;
+      *a.n_forks = missing > 0 ? 0 : forks;
+      if (missing > 0 && a.err) atomicAdd(a.err + 1, missing);
     }
     return;
   }
@@ -200,39 +207,10 @@ __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs 
     a.fresh[rank] = (int32_t)(p0 + __builtin_ctz(open));
 }
 
-// A wave per sequence: its new table entries and their counts, and its fork.
-__global__ void __launch_bounds__(kPageThreads) reserve_assign_kernel(ReserveArgs a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int b = (int)blockIdx.x * (kPageThreads / kWave) + uniform((int)threadIdx.x >> 6);
-  if (b >= a.batch || *a.short_of > 0) return;
-  const int want = a.need[b];
-  if (want == 0) return;
-  const RowStep r = row_step(a, b);
-  const int fork = want & kForkBit ? 1 : 0;
-  const int n = (want & ~kForkBit) - fork;
-  const int32_t* got = a.fresh + a.base[b];
-  int32_t* row = a.tables + b * a.stride;
-  for (int i = lane; i < n; i += kWave) {
-    const int page = got[fork + i];
-    row[r.first + i] = page;
-    a.refs[page] = 1;
-  }
-  if (fork && lane == 0) {
-    const int old = row[r.part], page = got[0];
-    row[r.part] = page;
-    a.refs[page] = 1;
-    atomicSub(a.refs + old, 1);
-    const int at = atomicAdd(a.n_forks, 1);  // the forks' order does not matter
-    a.fork_src[at] = old;
-    a.fork_dst[at] = page;
-    a.fork_rows[at] = r.rows;
-  }
-}
-
 // ----------------------------------------------------------------------------
-// Copies of pages in every layer: the page src[i] to dst[i], i < *count, the
-// first rows[i] rows of each (K|V, head) block or (rows null) all of it.  No
-// destination is a source.  Resident workgroups walk units of up to kCopyUnit
+// Copies of pages in every layer: the page src[i] to dst[i], i < *count; forks
+// (ROWS) the first rows[i] rows of each (K|V, head) block, to page
+// dst[dst_at[i]].  No destination is a source.  Resident workgroups walk units of up to kCopyUnit
 // bytes; a page's layer is one run of 2 Hkv 16 D elements.  Bound by HBM: every
 // byte is read and written once.
 struct CopyArgs {
@@ -241,6 +219,7 @@ struct CopyArgs {
   const int32_t* count;
   const int32_t* src;
   const int32_t* dst;
+  const int32_t* dst_at;
   const int32_t* rows;
   int32_t num_layers, num_pages, blocks;  // blocks: 2 Hkv
   int32_t block_bytes, row_bytes;
@@ -260,7 +239,7 @@ __device__ __forceinline__ void copy_pages(const CopyArgs& c, int64_t wg, int64_
     const int layer = rem / c.units;
     const int part = rem - layer * c.units;
     const int64_t from = (int64_t)layer * c.num_pages + uniform(c.src[i]);
-    const int64_t to = (int64_t)layer * c.num_pages + uniform(c.dst[i]);
+    const int64_t to = (int64_t)layer * c.num_pages + uniform(c.dst[ROWS ? c.dst_at[i] : i]);
     const int bytes = ROWS ? uniform(c.rows[i]) * c.row_bytes : c.block_bytes;
     const uint8_t* s = c.pool + from * page_bytes;
     uint8_t* d = c.pool + to * page_bytes;
@@ -284,7 +263,33 @@ __device__ __forceinline__ void copy_pages(const CopyArgs& c, int64_t wg, int64_
   }
 }
 
-__global__ void __launch_bounds__(kPageThreads) fork_rows_kernel(CopyArgs c) {
+// A wave per sequence: its new table entries and their counts.  Every workgroup:
+// its share of the forks' rows (the pages copied keep their rows, whoever
+// appends to them comes later on the stream).
+__global__ void __launch_bounds__(kPageThreads) reserve_assign_kernel(ReserveArgs a, CopyArgs c) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = uniform((int)threadIdx.x >> 6);
+  if (*a.short_of > 0) return;
+  for (int b = (int)blockIdx.x * (kPageThreads / kWave) + wave; b < a.batch;
+       b += (int)gridDim.x * (kPageThreads / kWave)) {
+    const int want = a.need[b];
+    if (want == 0) continue;
+    const RowStep r = row_step(a, b);
+    const int fork = want & kForkBit ? 1 : 0;
+    const int n = (want & ~kForkBit) - fork;
+    const int32_t* got = a.fresh + a.base[b];
+    int32_t* row = a.tables + b * a.stride;
+    for (int i = lane; i < n; i += kWave) {
+      const int page = got[fork + i];
+      row[r.first + i] = page;
+      a.refs[page] = 1;
+    }
+    if (fork && lane == 0) {
+      atomicSub(a.refs + row[r.part], 1);
+      row[r.part] = got[0];
+      a.refs[got[0]] = 1;
+    }
+  }
   copy_pages<true>(c, blockIdx.x, gridDim.x);
 }
 
@@ -615,7 +620,7 @@ int pagedattn_reserve_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layer
   a.need = take(batch_size);
   a.base = take(batch_size);
   a.fork_src = take(batch_size);
-  a.fork_dst = take(batch_size);
+  a.fork_rank = take(batch_size);
   a.fork_rows = take(batch_size);
   a.free_cnt = take(a.n_blocks);
   a.n_forks = take(64);
@@ -631,16 +636,14 @@ int pagedattn_reserve_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layer
                      a);
   rc = check_launch(who);
   if (rc) return rc;
-  hipLaunchKernelGGL(reserve_assign_kernel, dim3(waves), dim3(kPageThreads), 0, s, a);
-  rc = check_launch(who);
-  if (rc) return rc;
   c.count = a.n_forks;
   c.src = a.fork_src;
-  c.dst = a.fork_dst;
+  c.dst = a.fresh;
+  c.dst_at = a.fork_rank;
   c.rows = a.fork_rows;
   const int64_t units = (int64_t)batch_size * num_layers * c.units;
-  hipLaunchKernelGGL(fork_rows_kernel, dim3((unsigned)std::min<int64_t>(units, copy_grid())),
-                     dim3(kPageThreads), 0, s, c);
+  hipLaunchKernelGGL(reserve_assign_kernel, dim3((unsigned)std::min<int64_t>(units, copy_grid())),
+                     dim3(kPageThreads), 0, s, a, c);
   return check_launch(who);
 }
 

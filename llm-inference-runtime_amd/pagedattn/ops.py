@@ -549,6 +549,9 @@ def reserve_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, kv_lens: to
     because their lengths do not fit their table or their partial page is none of
     the pool's held ones; where the free pages do not suffice, nothing is changed
     and [1] grows by the pages missing."""
+    if _native("reserve", "pagedattn_reserve_pages", kv_pool, block_tables, kv_lens, new_lens,
+               ref_counts, kv_scales, error_flag) is None:
+        return
     n_layers, num_pages, hkv, d, scales = _whole_pool(kv_pool, kv_scales)
     bsz, max_pages = block_tables.shape if block_tables.dim() == 2 else (0, 0)
     device = _page_tables(block_tables, ref_counts, num_pages, error_flag, 2,
@@ -585,6 +588,9 @@ def release_window_pages(block_tables: torch.Tensor, kv_lens: torch.Tensor,
     """release_pages of the pages that lie wholly behind the window of the token
     at kv_lens[b] - 1 and past the sinks: neither it nor any later token sees
     them, and the windowed attention calls do not read their entries."""
+    if _native("release_window", "pagedattn_release_window_pages", block_tables, kv_lens,
+               ref_counts, window_left, num_sink_tokens, error_flag) is None:
+        return
     left, sinks = _window(window_left, num_sink_tokens)
     if left < 0:
         raise ValueError("release_window_pages needs a window (window_left >= 0)")

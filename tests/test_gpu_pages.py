@@ -11,6 +11,14 @@ from paged_cases import i32
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=["extension", "general"], autouse=True)
+def path(request, monkeypatch):
+    """Every test by the extension's calls and by the general path."""
+    if request.param == "general":
+        monkeypatch.setattr(pagedattn.ops, "_native", lambda *a: NotImplemented)
+
+
 POOLS = [(2, 3, 64, torch.bfloat16), (3, 1, 128, torch.float16), (1, 8, 128, torch.bfloat16),
          (2, 2, 64, torch.float8_e4m3fn), (1, 1, 16, torch.float8_e4m3fn)]
 
@@ -362,3 +370,36 @@ def test_calls_on_another_stream(gpu):
     side.synchronize()
     want.check(t, r, pool, scales)
     assert np.array_equal(remap.cpu().numpy(), remap_want)
+
+
+def test_the_extension_takes_the_plain_form(gpu, path, monkeypatch):
+    """And leaves what it does not take to the general path, which refuses or converts."""
+    assert pagedattn.ops._native("reserve", "reserve", *[None] * 7) is NotImplemented
+    pool, scales = make_pool(gpu, 9, POOLS[3])
+    t, r, n = i32([[-1, -1]], gpu), i32([0] * 9, gpu), i32([3], gpu)
+    took = []
+    real = pagedattn.ops._native
+    monkeypatch.setattr(pagedattn.ops, "_native",
+                        lambda *a: took.append(real(*a)) or took[-1])
+    pagedattn.reserve_pages(pool, t, n, i32([3], gpu), r, kv_scales=scales,
+                            error_flag=flags(gpu))
+    pagedattn.release_window_pages(t, n, r, 0)
+    assert t.tolist() == [[0, -1]] and r.tolist() == [1] + [0] * 8
+    assert len(took) == 2 and len({x is None for x in took}) == 1
+    for bad in (dict(pool=pool[:, :, :, :, :, ::2]), dict(pool=pool[0]), dict(t=t.long()),
+                dict(t=t.t()), dict(n=i32([3, 3], gpu)), dict(n=n.long()), dict(r=r[:5]),
+                dict(r=r.cpu()), dict(s=None), dict(s=scales.half()), dict(s=scales[:, :5]),
+                dict(new=i32([1, 1], gpu)), dict(err=flags(gpu, 1)), dict(err=flags(gpu).long())):
+        x = {**dict(pool=pool, t=t, n=n, new=None, r=r, s=scales, err=None), **bad}
+        with pytest.raises((ValueError, RuntimeError)):
+            pagedattn.reserve_pages(x["pool"], x["t"], x["n"], x["new"], x["r"],
+                                    kv_scales=x["s"], error_flag=x["err"])
+    with pytest.raises(pagedattn.PagedAttnError, match="dtype"):
+        pagedattn.reserve_pages(pool.float(), t, n, None, r)
+    for bad in (dict(t=t.long()), dict(n=n[:0]), dict(r=r.float()), dict(w=-1), dict(s=-1),
+                dict(err=flags(gpu).float())):
+        x = {**dict(t=t, n=n, r=r, w=3, s=0, err=None), **bad}
+        with pytest.raises(ValueError):
+            pagedattn.release_window_pages(x["t"], x["n"], x["r"], x["w"], x["s"],
+                                           error_flag=x["err"])
+    assert t.tolist() == [[0, -1]] and r.tolist() == [1] + [0] * 8
