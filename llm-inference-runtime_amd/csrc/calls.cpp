@@ -45,6 +45,7 @@ struct Entries {
   decltype(&pagedattn_page_scratch_bytes) page_scratch;
   decltype(&pagedattn_reserve_pages) reserve;
   decltype(&pagedattn_release_window_pages) release_window;
+  decltype(&pagedattn_decode_window_metadata) window_metadata;
 };
 Entries g_entry;
 PyObject* g_raw_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
@@ -228,11 +229,13 @@ bool arg_count(Py_ssize_t n, Py_ssize_t want) {
 }
 
 // decode_run(plan, q, pool, indices, indptr, last, batch, hq, hkv, d, scales,
-//            out, lse, return_lse, sm_scale, key, value, rope, positions[, holes])
-// holes: a windowed run's, over the lists of visible pages
+//            out, lse, return_lse, sm_scale, key, value, rope, positions[, holes,
+//            lists])
+// holes: a windowed run's, over the lists of visible pages; lists: None, or
+// (indices, indptr, window_left, sinks) to make them from, ahead of the run
 PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 20 && !arg_count(n, 19)) return nullptr;
+  if (n != 21 && !arg_count(n, 19)) return nullptr;
   auto* plan = static_cast<pagedattn_plan*>(PyLong_AsVoidPtr(a[0]));
   const int64_t bsz = PyLong_AsLongLong(a[6]), hq = PyLong_AsLongLong(a[7]),
                 hkv = PyLong_AsLongLong(a[8]), d = PyLong_AsLongLong(a[9]);
@@ -249,8 +252,21 @@ PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!meta(a[3], q->device(), -1, &indices, &n_ind) ||
       !meta(a[4], q->device(), bsz + 1, &indptr) || !meta(a[5], q->device(), bsz, &last))
     return general();
-  const int32_t* holes = nullptr;
-  if (n == 20 && a[19] != Py_None && !meta(a[19], q->device(), 4 * bsz, &holes)) return general();
+  const int32_t *holes = nullptr, *all_indices = nullptr, *all_indptr = nullptr;
+  int64_t n_all = 0;
+  int32_t window_left = 0, sinks = 0;
+  if (n == 21 && a[19] != Py_None && !meta(a[19], q->device(), 4 * bsz, &holes)) return general();
+  const bool lists = holes && a[20] != Py_None;
+  if (lists) {
+    PyObject* t = a[20];
+    if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 4 ||
+        !meta(PyTuple_GET_ITEM(t, 0), q->device(), -1, &all_indices, &n_all) ||
+        !meta(PyTuple_GET_ITEM(t, 1), q->device(), bsz + 1, &all_indptr))
+      return general();
+    window_left = (int32_t)PyLong_AsLong(PyTuple_GET_ITEM(t, 2));
+    sinks = (int32_t)PyLong_AsLong(PyTuple_GET_ITEM(t, 3));
+    if (PyErr_Occurred()) return nullptr;
+  }
   const bool append = a[15] != Py_None;
   const bool rope = a[17] != Py_None;
   const at::Tensor *k = nullptr, *v = nullptr;
@@ -288,12 +304,19 @@ PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t vs[2] = {append ? v->stride(0) : 0, append ? v->stride(1) : 0};
   Scratch scratch;
   scratch.get(plan, *q);
-  int rc;
+  int rc = 0;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_entry.decode_run(plan, holes, qp, q->stride(0), q->stride(1), code, kp, vp, ks[0], ks[1],
-                          vs[0], vs[1], rope, pos, (float)rope_scale, (float)rope_theta, pp,
-                          pool.code, scales, (int32_t)pool.pages, indices, (int32_t)n_ind, indptr,
-                          last, op, lp, (float)scale, scratch.ptr, scratch.bytes, stream);
+  if (lists)
+    rc = g_entry.window_metadata(all_indptr, all_indices, (int32_t)n_all, last, (int32_t)bsz,
+                                 window_left, sinks, const_cast<int32_t*>(indptr),
+                                 const_cast<int32_t*>(indices), (int32_t)n_ind,
+                                 const_cast<int32_t*>(holes), stream);
+  if (!rc)
+    rc = g_entry.decode_run(plan, holes, qp, q->stride(0), q->stride(1), code, kp, vp, ks[0], ks[1],
+                            vs[0], vs[1], rope, pos, (float)rope_scale, (float)rope_theta, pp,
+                            pool.code, scales, (int32_t)pool.pages, indices, (int32_t)n_ind,
+                            indptr, last, op, lp, (float)scale, scratch.ptr, scratch.bytes,
+                            stream);
   Py_END_ALLOW_THREADS
   return rc ? PyLong_FromLong(rc) : o.result();
   END_HANDLE_TH_ERRORS
@@ -638,6 +661,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   e.reserve = reinterpret_cast<decltype(e.reserve)>(at("pagedattn_reserve_pages"));
   e.release_window =
       reinterpret_cast<decltype(e.release_window)>(at("pagedattn_release_window_pages"));
+  e.window_metadata =
+      reinterpret_cast<decltype(e.window_metadata)>(at("pagedattn_decode_window_metadata"));
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: missing entry point");
     return nullptr;

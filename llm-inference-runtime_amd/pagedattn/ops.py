@@ -1132,16 +1132,18 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         entry = ("pagedattn_decode_run" if append_key is None else
                  "pagedattn_decode_run_append" if rope is None else
                  "pagedattn_decode_run_rope_append")
-        indices, indptr, holes = self._indices, self._indptr, self._holes
+        indices, indptr, holes, lists = self._indices, self._indptr, self._holes, None
         if holes is not None:
-            if not self._lists_made:
-                self._make_lists()
             indices, indptr = self._seen_indices, self._seen_indptr
+            if not self._lists_made:
+                lists = (self._indices, self._indptr, self._window_left, self._sinks)
         r = _native("decode_run", entry, self._plan.handle, q, paged_kv_cache, indices, indptr,
                     self._last, self._bsz, self._hq, self._hkv, self._d, kv_scales, out, lse,
-                    return_lse, scale, append_key, append_value, rope, positions, holes)
+                    return_lse, scale, append_key, append_value, rope, positions, holes, lists)
         if r is not NotImplemented:
             return r
+        if lists is not None:
+            self._make_lists()
         num_pages, _, _ = _check_pool(paged_kv_cache, self._hkv, self._d, self._kv_layout)
         _check_rows(q, "q", self._hq, self._d)
         if q.shape[0] != self._bsz:

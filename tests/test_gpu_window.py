@@ -22,6 +22,13 @@ from paged_cases import i32, random_tables, require_shared_plans, strided_rows, 
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture
+def general(monkeypatch):
+    """The calls' general path: the extension takes nothing."""
+    monkeypatch.setattr(pagedattn.ops, "_native", lambda *a: NotImplemented)
+
+
 HEADS = [(32, 4, 64), (32, 8, 128), (8, 8, 64), (16, 1, 128)]
 
 
@@ -519,3 +526,24 @@ def test_a_window_of_the_largest_size(gpu):
     for kind in ("host", "device"):
         w = plan_decode(gpu, one, heads, dtype, window, sinks, kind)
         check(*w.run(q, pool, return_lse=True), reference(one, pool, scales, q, window, sinks))
+
+
+@pytest.mark.parametrize("kind", ["host", "device"])
+def test_decode_by_the_general_path(gpu, kind, request):
+    """The same bits as the extension's call, with RoPE and append and without."""
+    heads, dtype, window, sinks = HEADS[0], torch.float16, 60, 17
+    meta, pool, _, q = make(gpu, [n - 1 for n in LENS], [1] * len(LENS), heads, dtype, False,
+                            window, sinks, 1)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(1)
+    k, v = (torch.randn((len(LENS), 4, 64), generator=g, device=gpu).to(dtype) for _ in range(2))
+    got = []
+    for native in (True, False):
+        if not native:
+            request.getfixturevalue("general")
+        p = pool.clone()
+        w = plan_decode(gpu, meta, heads, dtype, window, sinks, kind)
+        out, lse = w.run(q, p, return_lse=True)
+        fused = w.run(q, p, append_key=k, append_value=v, rope=(1.0, 1e4))
+        got.append((out, lse, fused, p.view(torch.int16)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
