@@ -22,6 +22,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/TensorOptions.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/util/Exception.h>
@@ -45,6 +46,7 @@ struct Entries {
   decltype(&pagedattn_page_scratch_bytes) page_scratch;
   decltype(&pagedattn_reserve_pages) reserve;
   decltype(&pagedattn_release_window_pages) release_window;
+  decltype(&pagedattn_compact_pages) compact;
   decltype(&pagedattn_decode_window_metadata) window_metadata;
 };
 Entries g_entry;
@@ -544,6 +546,7 @@ struct Tables {
     if (numel) *numel = t->numel();
     return true;
   }
+  // lens_o null: a call without lengths
   bool get(PyObject* tables_o, PyObject* lens_o, PyObject* refs_o, PyObject* flag_o, int64_t flags) {
     const at::Tensor* t = plain(tables_o);
     if (!t || !t->is_cuda() || t->dim() != 2 || t->scalar_type() != at::kInt || t->size(0) < 1 ||
@@ -556,7 +559,8 @@ struct Tables {
     stride = std::max(t->stride(0), width);
     tables = static_cast<int32_t*>(t->data_ptr());
     int32_t* l = nullptr;
-    if (!ints(lens_o, batch, &l) || !ints(refs_o, -1, &refs, &pages) || pages > INT32_MAX)
+    if ((lens_o && !ints(lens_o, batch, &l)) || !ints(refs_o, -1, &refs, &pages) ||
+        pages > INT32_MAX)
       return false;
     lens = l;
     if (flag_o == Py_None) return true;
@@ -565,45 +569,89 @@ struct Tables {
   }
 };
 
+// The pool of all layers, [L, P, 2, Hkv, 16, D], with its scales (e4m3).
+struct WholePool {
+  void* ptr = nullptr;
+  float* scales = nullptr;
+  int code = -1;
+  int32_t layers = 0, hkv = 0, d = 0;
+  bool get(PyObject* o, PyObject* scales_o, const Tables& x) {
+    const at::Tensor* t = plain(o);
+    if (!t || t->device() != x.device || t->dim() != 6 || t->size(2) != 2 ||
+        t->size(4) != kPageSize || !t->is_contiguous() || t->size(1) != x.pages ||
+        t->size(0) > INT32_MAX || t->size(3) > INT32_MAX || t->size(5) > INT32_MAX)
+      return false;
+    ptr = t->data_ptr();
+    layers = (int32_t)t->size(0);
+    hkv = (int32_t)t->size(3);
+    d = (int32_t)t->size(5);
+    code = t->scalar_type() == at::kFloat8_e4m3fn ? PAGEDATTN_E4M3 : code16(*t);
+    if (code != PAGEDATTN_E4M3) return code >= 0;
+    const at::Tensor* s = plain(scales_o);
+    if (!s || s->device() != x.device || s->scalar_type() != at::kFloat || s->dim() != 4 ||
+        s->size(0) != layers || s->size(1) != x.pages || s->size(2) != 2 || s->size(3) != hkv ||
+        !s->is_contiguous())
+      return false;
+    scales = static_cast<float*>(s->data_ptr());
+    return true;
+  }
+};
+
+// A page call's scratch, from torch's allocator on the current device.
+struct PageScratch {
+  size_t bytes;
+  c10::DataPtr mem;
+  explicit PageScratch(const Tables& x)
+      : bytes(g_entry.page_scratch((int32_t)x.pages, (int32_t)x.batch, (int32_t)x.width)),
+        mem(c10::GetAllocator(c10::DeviceType::CUDA)->allocate(std::max<size_t>(bytes, 256))) {}
+};
+
 // reserve(pool, tables, kv_lens, new_lens, ref_counts, scales, flag)
 PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arg_count(n, 7)) return nullptr;
   Tables x;
-  const at::Tensor* pool = plain(a[0]);
-  if (!pool || !x.get(a[1], a[2], a[4], a[6], 2) || pool->device() != x.device ||
-      pool->dim() != 6 || pool->size(2) != 2 || pool->size(4) != kPageSize ||
-      !pool->is_contiguous() || pool->size(1) != x.pages || pool->size(0) > INT32_MAX ||
-      pool->size(3) > INT32_MAX || pool->size(5) > INT32_MAX)
-    return general();
-  const int code = pool->scalar_type() == at::kFloat8_e4m3fn ? PAGEDATTN_E4M3 : code16(*pool);
-  if (code < 0) return general();
+  WholePool pool;
   int32_t* added = nullptr;
-  if (a[3] != Py_None && !x.ints(a[3], x.batch, &added)) return general();
-  float* scales = nullptr;
-  if (code == PAGEDATTN_E4M3) {
-    const at::Tensor* t = plain(a[5]);
-    if (!t || t->device() != x.device || t->scalar_type() != at::kFloat || t->dim() != 4 ||
-        t->size(0) != pool->size(0) || t->size(1) != x.pages || t->size(2) != 2 ||
-        t->size(3) != pool->size(3) || !t->is_contiguous())
-      return general();
-    scales = static_cast<float*>(t->data_ptr());
-  }
+  if (!x.get(a[1], a[2], a[4], a[6], 2) || !pool.get(a[0], a[5], x) ||
+      (a[3] != Py_None && !x.ints(a[3], x.batch, &added)))
+    return general();
   void* stream;
   if (!raw_stream(x.device, &stream)) return nullptr;
   const c10::DeviceGuard guard(x.device);
-  const size_t bytes = g_entry.page_scratch((int32_t)x.pages, (int32_t)x.batch, (int32_t)x.width);
-  const c10::DataPtr scratch =
-      c10::GetAllocator(c10::DeviceType::CUDA)->allocate(std::max<size_t>(bytes, 256));
-  void* pp = pool->data_ptr();
+  const PageScratch scratch(x);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_entry.reserve(pp, code, (int32_t)pool->size(0), (int32_t)x.pages, (int32_t)pool->size(3),
-                       (int32_t)pool->size(5), kPageSize, scales, x.tables, x.stride,
-                       (int32_t)x.width, x.lens, added, (int32_t)x.batch, x.refs, x.flag,
-                       scratch.get(), bytes, stream);
+  rc = g_entry.reserve(pool.ptr, pool.code, pool.layers, (int32_t)x.pages, pool.hkv, pool.d,
+                       kPageSize, pool.scales, x.tables, x.stride, (int32_t)x.width, x.lens, added,
+                       (int32_t)x.batch, x.refs, x.flag, scratch.mem.get(), scratch.bytes, stream);
   Py_END_ALLOW_THREADS
   return done(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// compact(pool, tables, ref_counts, scales, flag): remap
+PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 5)) return nullptr;
+  Tables x;
+  WholePool pool;
+  if (!x.get(a[1], nullptr, a[2], a[4], 1) || !pool.get(a[0], a[3], x) || x.pages < 1)
+    return general();
+  void* stream;
+  if (!raw_stream(x.device, &stream)) return nullptr;
+  const c10::DeviceGuard guard(x.device);
+  const PageScratch scratch(x);
+  at::Tensor remap = at::empty({x.pages}, at::TensorOptions().dtype(at::kInt).device(x.device));
+  auto* rp = static_cast<int32_t*>(remap.data_ptr());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_entry.compact(pool.ptr, pool.code, pool.layers, (int32_t)x.pages, pool.hkv, pool.d,
+                       kPageSize, pool.scales, x.tables, x.stride, (int32_t)x.width,
+                       (int32_t)x.batch, x.refs, rp, x.flag, scratch.mem.get(), scratch.bytes,
+                       stream);
+  Py_END_ALLOW_THREADS
+  return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(remap);
   END_HANDLE_TH_ERRORS
 }
 
@@ -661,6 +709,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   e.reserve = reinterpret_cast<decltype(e.reserve)>(at("pagedattn_reserve_pages"));
   e.release_window =
       reinterpret_cast<decltype(e.release_window)>(at("pagedattn_release_window_pages"));
+  e.compact = reinterpret_cast<decltype(e.compact)>(at("pagedattn_compact_pages"));
   e.window_metadata =
       reinterpret_cast<decltype(e.window_metadata)>(at("pagedattn_decode_window_metadata"));
   if (!ok) {
@@ -683,6 +732,7 @@ PyMethodDef kMethods[] = {
     {"append_amax", FAST(append_amax), nullptr},
     {"axes_append", FAST(axes_append), nullptr},
     {"reserve", FAST(reserve), nullptr},
+    {"compact", FAST(compact), nullptr},
     {"release_window", FAST(release_window), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -646,6 +646,10 @@ def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, ref_counts:
     in place.  Returns remap [num_pages] int32: each page's new id, -1 for free
     ones, for tables kept elsewhere (a prefix cache).  error_flag counts entries
     that name a page outside the pool or a free one; they stay as they are."""
+    remap = _native("compact", "pagedattn_compact_pages", kv_pool, block_tables, ref_counts,
+                    kv_scales, error_flag)
+    if remap is not NotImplemented:
+        return remap
     n_layers, num_pages, hkv, d, scales = _whole_pool(kv_pool, kv_scales)
     device = _page_tables(block_tables, ref_counts, num_pages, error_flag, 1)
     if kv_pool.device != device:
