@@ -21,32 +21,71 @@ namespace pa {
 
 constexpr int kPagesPerBlock = 4096;
 constexpr int kPageThreads = 256;
-constexpr int kPagesPerThread = kPagesPerBlock / kPageThreads;
+constexpr int kPageWaves = kPageThreads / kWave;
+constexpr int kPageSteps = kPagesPerBlock / kPageThreads;
 
-// ref_counts of kPagesPerThread consecutive pages (a thread's share of a block)
-// as bits: bit i set where the count of page p0 + i is not 0.  Pages past the
-// pool count as `past`.
-__device__ __forceinline__ uint32_t live_bits(const int32_t* refs, int64_t p0, int num_pages,
-                                              bool past) {
-  uint32_t m = 0;
-  if (p0 + kPagesPerThread <= num_pages && aligned16(refs)) {
-    // whole 16-byte loads (p0 is a multiple of 16 pages)
-    int4 v[kPagesPerThread / 4];
+// Which of a block's pages are held.  Wave w has pages 1024 w to 1024 w + 1023 of
+// it: bit `lane` of m[k] is page 1024 w + 64 k + lane.  Pages past the pool count
+// as `past`.  One coalesced load a step, all in flight at once.
+struct Held {
+  uint64_t m[kPageSteps];
+  int64_t page0;  // the wave's first page
+
+  __device__ __forceinline__ void load(const int32_t* refs, int block, int num_pages, bool past) {
+    const int lane = threadIdx.x & (kWave - 1);
+    page0 = (int64_t)block * kPagesPerBlock +
+            uniform((int)threadIdx.x >> 6) * (kPagesPerBlock / kPageWaves);
+    int v[kPageSteps];
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread / 4; ++i)
-      v[i] = reinterpret_cast<const int4*>(refs + p0)[i];
+    for (int k = 0; k < kPageSteps; ++k) {
+      const int64_t p = page0 + k * kWave + lane;
+      v[k] = past ? 1 : 0;
+      if (p < num_pages) v[k] = refs[p];
+    }
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread / 4; ++i)
-      m |= ((v[i].x != 0 ? 1u : 0u) | (v[i].y != 0 ? 2u : 0u) | (v[i].z != 0 ? 4u : 0u) |
-            (v[i].w != 0 ? 8u : 0u))
-           << (4 * i);
-    return m;
+    for (int k = 0; k < kPageSteps; ++k) m[k] = __builtin_amdgcn_ballot_w64(v[k] != 0);
   }
-  for (int i = 0; i < kPagesPerThread; ++i) {
-    const bool in = p0 + i < num_pages;
-    if (in ? refs[p0 + i] != 0 : past) m |= 1u << i;
+  __device__ __forceinline__ int count() const {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kPageSteps; ++k) n += (int)__builtin_popcountll(m[k]);
+    return n;
   }
-  return m;
+  // those with a page id below `line`
+  __device__ __forceinline__ int count_below(int64_t line) const {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kPageSteps; ++k) {
+      const int64_t d = line - (page0 + k * kWave);
+      const uint64_t in = d >= kWave ? ~0ull : d > 0 ? (1ull << (int)d) - 1 : 0ull;
+      n += (int)__builtin_popcountll(m[k] & in);
+    }
+    return n;
+  }
+};
+
+// Bits of m below the lane's own.
+__device__ __forceinline__ int bits_below(uint64_t m) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+}
+
+// Sum of a wave-uniform value over the workgroup's waves; *before gets that of
+// the waves before this one.
+__device__ __forceinline__ int waves_sum(int v, int* red, int* before) {
+  const int wave = uniform((int)threadIdx.x >> 6);
+  __syncthreads();  // the last use of `red` is over
+  if ((threadIdx.x & (kWave - 1)) == 0) red[wave] = v;
+  __syncthreads();
+  int all = 0, mine = 0;
+#pragma unroll
+  for (int w = 0; w < kPageWaves; ++w) {
+    const int x = red[w];
+    all += x;
+    mine += w < wave ? x : 0;
+  }
+  *before = mine;
+  return all;
 }
 
 __device__ __forceinline__ int block_sum(int v, int* red) {
@@ -125,11 +164,11 @@ __global__ void __launch_bounds__(kPageThreads) reserve_count_kernel(ReserveArgs
   __shared__ int red[kPageThreads / kWave];
   const int lane = threadIdx.x & (kWave - 1);
   if ((int)blockIdx.x < a.n_blocks) {
-    const int64_t p0 =
-        (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-    const uint32_t live = live_bits(a.refs, p0, a.num_pages, true);
-    const int n = block_sum(kPagesPerThread - __builtin_popcount(live), red);
-    if (threadIdx.x == 0) a.free_cnt[blockIdx.x] = n;
+    Held held;
+    held.load(a.refs, (int)blockIdx.x, a.num_pages, true);
+    int before;
+    const int n = waves_sum(held.count(), red, &before);
+    if (threadIdx.x == 0) a.free_cnt[blockIdx.x] = kPagesPerBlock - n;
     return;
   }
   const int b = ((int)blockIdx.x - a.n_blocks) * (kPageThreads / kWave) +
@@ -193,18 +232,25 @@ __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs 
     return;
   }
   // the block's pages are on their way while the counts are summed
-  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-  uint32_t open = ~live_bits(a.refs, p0, a.num_pages, true) & ((1u << kPagesPerThread) - 1);
+  Held held;
+  held.load(a.refs, (int)blockIdx.x, a.num_pages, true);
   int wanted = 0;
   for (int b = (int)threadIdx.x; b < a.batch; b += kPageThreads) wanted += a.need[b] & ~kForkBit;
   wanted = block_sum(wanted, red);
   const int before = array_sum(a.free_cnt, (int)blockIdx.x, red);
   if (before >= wanted) return;  // uniform
-  int total;
-  __syncthreads();
-  int rank = before + block_excl_scan<kPageThreads>(__builtin_popcount(open), &total, red);
-  for (; open && rank < wanted; open &= open - 1, ++rank)
-    a.fresh[rank] = (int32_t)(p0 + __builtin_ctz(open));
+  int held_before;
+  waves_sum(held.count(), red, &held_before);
+  // free pages before the wave's first
+  int rank = before + uniform((int)threadIdx.x >> 6) * (kPagesPerBlock / kPageWaves) - held_before;
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int k = 0; k < kPageSteps; ++k) {
+    const uint64_t open = ~held.m[k];
+    const int at = rank + bits_below(open);
+    if (((open >> lane) & 1) && at < wanted) a.fresh[at] = (int32_t)(held.page0 + k * kWave + lane);
+    rank += (int)__builtin_popcountll(open);
+  }
 }
 
 // ----------------------------------------------------------------------------
@@ -405,56 +451,89 @@ struct CompactArgs {
 constexpr int32_t kStays = -1, kFree = -2;
 
 __global__ void __launch_bounds__(kPageThreads) compact_count_kernel(CompactArgs a) {
-  __shared__ int red[kPageThreads / kWave];
-  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-  const int n = block_sum(__builtin_popcount(live_bits(a.refs, p0, a.num_pages, false)), red);
+  __shared__ int red[kPageWaves];
+  Held held;
+  held.load(a.refs, (int)blockIdx.x, a.num_pages, false);
+  int before;
+  const int n = waves_sum(held.count(), red, &before);
   if (threadIdx.x == 0) a.live_cnt[blockIdx.x] = n;
 }
 
+// COUNTS: the blocks' counts come from compact_count_kernel.  Pools of up to
+// kOwnBlocks blocks are counted by every workgroup itself, which saves a launch.
+constexpr int kOwnBlocks = 4;
+
+template <bool COUNTS>
 __global__ void __launch_bounds__(kPageThreads) compact_rank_kernel(CompactArgs a) {
-  __shared__ int red[kPageThreads / kWave];
-  // this block's pages are on their way while the counts are summed
-  const int64_t p0 = (int64_t)blockIdx.x * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-  const uint32_t live = live_bits(a.refs, p0, a.num_pages, false);
-  int all = 0, mine = 0;
-  for (int i = (int)threadIdx.x; i < a.n_blocks; i += kPageThreads) {
-    const int n = a.live_cnt[i];
-    all += n;
-    mine += i < (int)blockIdx.x ? n : 0;
+  __shared__ int red[kPageWaves];
+  const int blk = (int)blockIdx.x;
+  Held held;  // on its way while the counts are summed
+  held.load(a.refs, blk, a.num_pages, false);
+  // live pages in all, and in the blocks before this one
+  int n_live, before_blk, unused;
+  int own[kOwnBlocks];  // the wave's share of every block's
+  if constexpr (COUNTS) {
+    int all = 0, mine = 0;
+    for (int i = (int)threadIdx.x; i < a.n_blocks; i += kPageThreads) {
+      const int n = a.live_cnt[i];
+      all += n;
+      mine += i < blk ? n : 0;
+    }
+    n_live = block_sum(all, red);
+    before_blk = block_sum(mine, red);
+  } else {
+    int all = 0, mine = 0;
+#pragma unroll
+    for (int i = 0; i < kOwnBlocks; ++i) {
+      own[i] = 0;
+      if (i < a.n_blocks) {
+        Held other;
+        other.load(a.refs, i, a.num_pages, false);
+        own[i] = other.count();
+      }
+      all += own[i];
+      mine += i < blk ? own[i] : 0;
+    }
+    n_live = waves_sum(all, red, &unused);
+    before_blk = waves_sum(mine, red, &unused);
   }
-  const int n_live = block_sum(all, red);
-  const int before_blk = block_sum(mine, red);
   // live pages below n_live, which stay
   const int line_blk = min(n_live / kPagesPerBlock, a.n_blocks - 1);
-  const int64_t l0 = (int64_t)line_blk * kPagesPerBlock + (int64_t)threadIdx.x * kPagesPerThread;
-  uint32_t below = live_bits(a.refs, l0, a.num_pages, false);
-  const int64_t inside = n_live - l0;  // of this thread's pages, those below the line
-  below &= inside >= kPagesPerThread ? ~0u : inside > 0 ? (1u << (int)inside) - 1 : 0u;
-  int under = __builtin_popcount(below);
-  for (int i = (int)threadIdx.x; i < line_blk; i += kPageThreads) under += a.live_cnt[i];
-  const int stay = block_sum(under, red);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  Held at_line;
+  at_line.load(a.refs, line_blk, a.num_pages, false);
+  int stay = at_line.count_below(n_live);
+  if constexpr (COUNTS) {
+    stay = waves_sum(stay, red, &unused);
+    stay += array_sum(a.live_cnt, line_blk, red);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kOwnBlocks; ++i) stay += i < line_blk ? own[i] : 0;
+    stay = waves_sum(stay, red, &unused);
+  }
+  if (blk == 0 && threadIdx.x == 0) {
     *a.n_live = n_live;
     *a.n_moves = n_live - stay;
   }
-  int total;
-  __syncthreads();
-  int before = before_blk +
-               block_excl_scan<kPageThreads>(__builtin_popcount(live), &total, red);
-  for (int i = 0; i < kPagesPerThread; ++i) {
-    const int64_t p = p0 + i;
-    if (p >= a.num_pages) break;
-    const bool is_live = (live >> i) & 1;
+  int before;  // live pages before the wave's first, then before each step's
+  waves_sum(held.count(), red, &before);
+  before += before_blk;
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int k = 0; k < kPageSteps; ++k) {
+    const int64_t p = held.page0 + k * kWave + lane;
+    const bool is_live = (held.m[k] >> lane) & 1;
+    const int rank = before + bits_below(held.m[k]);
+    before += (int)__builtin_popcountll(held.m[k]);
+    if (p >= a.num_pages) continue;
     int move = is_live ? kStays : kFree;
     if (is_live && p >= n_live) {
-      move = before - stay;
+      move = rank - stay;
       a.src[move] = (int32_t)p;
     } else if (!is_live && p < n_live) {
-      a.dst[(int)p - before] = (int32_t)p;
+      a.dst[(int)p - rank] = (int32_t)p;
     }
     a.move[p] = move;
     if (move < 0) a.remap[p] = is_live ? (int32_t)p : -1;
-    before += is_live ? 1 : 0;
   }
 }
 
@@ -742,11 +821,15 @@ int pagedattn_compact_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layer
   a.n_live = at;
   a.n_moves = at + 1;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)a.n_blocks), dim3(kPageThreads), 0, s,
-                     a);
-  rc = check_launch(who);
-  if (rc) return rc;
-  hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)a.n_blocks), dim3(kPageThreads), 0, s, a);
+  const bool counts = a.n_blocks > kOwnBlocks;
+  if (counts) {
+    hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)a.n_blocks), dim3(kPageThreads), 0, s,
+                       a);
+    rc = check_launch(who);
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(counts ? compact_rank_kernel<true> : compact_rank_kernel<false>,
+                     dim3((unsigned)a.n_blocks), dim3(kPageThreads), 0, s, a);
   rc = check_launch(who);
   if (rc) return rc;
   c.count = a.n_moves;

@@ -304,7 +304,8 @@ def test_share(gpu, on_device):
 
 @pytest.mark.parametrize("shape", POOLS)
 @pytest.mark.parametrize("num_pages,live", [(1, 1.0), (1, 0.0), (37, 0.4), (4096, 0.9),
-                                            (4097, 0.5), (9001, 0.1), (600, 1.0)])
+                                            (4097, 0.5), (9001, 0.1), (600, 1.0),
+                                            (65536, 0.3)])
 def test_compact(gpu, shape, num_pages, live):
     rng = np.random.default_rng(num_pages)
     refs = (rng.random(num_pages) < live) * rng.integers(1, 4, num_pages)
@@ -321,6 +322,21 @@ def test_compact(gpu, shape, num_pages, live):
     assert np.array_equal(remap.cpu().numpy(), want_remap) and err.item() == 0
     n = int((refs > 0).sum())
     assert bool((r[:n] > 0).all()) and not r[n:].any()
+
+
+@pytest.mark.parametrize("num_pages", [65537, 300001])
+def test_compact_of_many_pages(gpu, num_pages):
+    """Past the pools whose blocks every workgroup counts itself."""
+    rng = np.random.default_rng(num_pages)
+    refs = (rng.random(num_pages) < 0.4).astype(int)
+    tables = rng.choice(np.flatnonzero(refs), (3, 700))
+    pool, _ = make_pool(gpu, num_pages, (1, 1, 16, torch.float16))
+    want = Oracle(tables, refs, pool, None)
+    t, r, err = i32(tables, gpu), i32(refs, gpu), flags(gpu, 1)
+    remap = pagedattn.compact_pages(pool, t, r, error_flag=err)
+    want_remap, _ = want.compact()
+    want.check(t, r, pool, None)
+    assert np.array_equal(remap.cpu().numpy(), want_remap) and err.item() == 0
 
 
 def test_compact_leaves_entries_of_no_held_page(gpu):
