@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <queue>
+#include <new>
 #include <vector>
 
 #include "plan_internal.h"
@@ -416,7 +417,7 @@ int pagedattn_decode_plan_window(pagedattn_plan* plan, const int32_t* kv_indptr_
                                  int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
                                  int32_t page_size, int32_t split_pages, int32_t window_left,
                                  int32_t sinks, void* workspace, size_t workspace_bytes,
-                                 void* stream) {
+                                 void* stream) try {
   const char* who = "decode_plan";
   if (!plan) return set_error(PAGEDATTN_ERR_INVALID, "%s: null plan", who);
   plan->mode = kPlanNone;
@@ -441,6 +442,9 @@ int pagedattn_decode_plan_window(pagedattn_plan* plan, const int32_t* kv_indptr_
   return pagedattn_decode_plan(plan, listed.data(), kv_last_page_len_host, batch_size,
                                num_qo_heads, num_kv_heads, head_dim, page_size, split_pages,
                                workspace, workspace_bytes, stream);
+} catch (const std::bad_alloc&) {
+  return set_error(PAGEDATTN_ERR_INVALID, "decode_plan: no host memory for %d sequences",
+                   batch_size);
 }
 
 int pagedattn_decode_plan(pagedattn_plan* plan, const int32_t* kv_indptr_host,

@@ -11,8 +11,10 @@
 // pages and a rank by prefix sums, without a free list to keep in order;
 // reading 4 bytes a page, 0.4 MB for 100 000 pages, costs less than a launch.
 //
-// Bounds: the metadata kernels by launch and load latency (two or three
-// dependent loads each), the copies by HBM bandwidth.
+// Bounds: the metadata kernels by launch and load latency (two to four dependent
+// loads each: 512 rows over 100 000 pages 7.0, 4.3, 5.2 us for reserve's three
+// launches, 3.8 us for the release behind a window; 32 rows over 4000 pages 3.6,
+// 3.6, 5.8 and 2.8 us), the copies by HBM bandwidth.
 #include <algorithm>
 
 #include "common.h"
@@ -431,7 +433,10 @@ __global__ void __launch_bounds__(kPageThreads) share_pages_kernel(ShareArgs a) 
 // ----------------------------------------------------------------------------
 // compact: the n live pages move to ids [0, n).  Those already there stay; the
 // k-th live page at or past n goes to the k-th free page below n, so no
-// destination is a source and one launch can copy them all.
+// destination is a source and one launch can copy them all.  4950 pages of 4 layers
+// x 32 KiB, 1.3 GB read and written: 256 us, 5.1 TB/s (a large copy moves 4.8);
+// the ranks before it 12 us.  Pages are copied layer by layer in units of 16 KiB, 4
+// loads of 16 bytes a thread at once, by one resident set of workgroups.
 struct CompactArgs {
   int32_t* refs;
   int32_t num_pages, n_blocks;

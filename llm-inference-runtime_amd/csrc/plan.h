@@ -124,7 +124,8 @@ inline __host__ __device__ bool prefill_split_pays(int t_max, int len, int64_t c
 // position p_lo on see, up to kv_end: the `sink_pages` first, and those from
 // `shift` pages further on.  A windowed q-tile walks them four to a KV tile, `total`
 // tiles in all: aligned tiles would read a tile for a few sinks and half a tile
-// ahead of the window (window 1023, 16 sinks: 18.5 against 17.5 tiles).
+// ahead of the window (prompts of 14 576 tokens, window 1023, 16 sinks: 321 us with
+// aligned tiles, 309 us with these).
 struct WindowTiles {
   int sink_pages, shift, total;
 };

@@ -9,6 +9,7 @@
 #include <climits>
 #include <cstdlib>
 #include <cstring>
+#include <new>
 #include <vector>
 
 #include "plan_internal.h"
@@ -114,7 +115,7 @@ int pagedattn_prefill_plan_window(pagedattn_plan* plan, const int32_t* qo_indptr
                                   int32_t batch_size, int32_t num_qo_heads,
                                   int32_t num_kv_heads, int32_t head_dim,
                                   int32_t page_size, int32_t window_left, int32_t sinks,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
+                                  void* workspace, size_t workspace_bytes, void* stream) try {
   const char* who = "prefill_plan";
   if (!plan) return set_error(PAGEDATTN_ERR_INVALID, "%s: null plan", who);
   plan->mode = kPlanNone;
@@ -253,6 +254,9 @@ int pagedattn_prefill_plan_window(pagedattn_plan* plan, const int32_t* qo_indptr
   finish(plan);
   if (cut) set_split(plan, lay, (int64_t)pieces.size(), (int64_t)pieces.size());
   return PAGEDATTN_OK;
+} catch (const std::bad_alloc&) {
+  return set_error(PAGEDATTN_ERR_INVALID, "prefill_plan: no host memory for %d sequences",
+                   batch_size);
 }
 
 int pagedattn_prefill_plan_device(pagedattn_plan* plan, int32_t batch_size,

@@ -9,9 +9,10 @@
 // left as they are.
 //
 // Bound by HBM for prompts (each row read once, q and k rows written once, k and
-// v rows written to their pages) and by one load-to-store chain for a decode
-// step's rows.  The work is split as in the RoPE + append of one position
-// (misc.hip): a workgroup owns T tokens; 8 lanes (fewer where a head has fewer
+// v rows written to their pages: 21 181 tokens of 32/8 heads, D = 128, 564 MB in
+// 100 us, 5.6 TB/s, where a large copy moves 4.8) and by one load-to-store chain
+// for a decode step's rows (33 of 32/4 heads, D = 64: 4.4 us).  The work is split as in the RoPE + append of one position
+// (misc.hip): a workgroup owns T tokens (launch_rope_axes); 8 lanes (fewer where a head has fewer
 // chunk pairs) work a head, each with two 16-byte chunks; the cosines and sines
 // are evaluated once per (token, frequency), one per lane, into LDS while the first
 // rows are on their way.
@@ -27,6 +28,9 @@ constexpr int kAxesFreqs = 64;   // frequencies of a workgroup (8 chunk pairs)
 constexpr int kAxesBatch = 4;    // heads a thread has in flight
 constexpr int kAxesTokens = 16;  // tokens of a workgroup at most
 constexpr int kAxesThreads = 256;
+constexpr int kAxesSpread = 512;   // workgroups before a token shares one
+constexpr int kAxesGroups = 1024;  // workgroups left by more than 4 tokens each
+constexpr int kAxesFewLanes = 96;  // of a token
 
 struct RopeAxesArgs {
   AppendArgs a;  // cache null: q and k only
@@ -246,10 +250,20 @@ static int launch_rope_axes(const char* who, RopeAxesArgs r, bool bf16, bool app
   const int pairs = std::min(r.a.d / 16, kAxesFreqs / 8);
   r.c_shift = 0;
   while ((1 << r.c_shift) < pairs) ++r.c_shift;
-  // tokens per workgroup: as many as one batch of loads covers
+  // tokens per workgroup: as many as one batch of loads covers, up to 4; one while
+  // that makes two workgroups a CU or fewer (512 tokens of 8/1 heads, D = 128, 3.7
+  // against 4.7 us with 4, of 32/4, D = 64, 3.7 against 5.2); and for many tokens of
+  // few heads as many as leave four workgroups a CU, up to 16, which hide their
+  // prologue better (8/1, D = 128: 8192 tokens 9.7 us with 8, 11.1 with 4; 65536 58.5
+  // us with 16, 69.2 with 4; 4/1, D = 64, 65536 26.6 and 40.4).  12/2 heads, 128
+  // lanes a token, gain less (65536 109.8 and 117.6, 4096 13.0 and 8.5) and stay
+  // below the line.
   const int64_t lanes = ((int64_t)r.hq + (append ? 2 : 1) * (int64_t)r.a.hkv) << r.c_shift;
-  r.tokens = (int)std::min<int64_t>(
-      4, std::max<int64_t>(1, kAxesThreads * kAxesBatch / 2 / std::max<int64_t>(lanes, 1)));
+  const int64_t batch = kAxesThreads * kAxesBatch / 2 / std::max<int64_t>(lanes, 1);
+  r.tokens = (int)std::max<int64_t>(
+      1, std::min<int64_t>({4, batch, r.a.nnz / kAxesSpread}));
+  if (lanes <= kAxesFewLanes)
+    r.tokens = std::max(r.tokens, std::min(kAxesTokens, r.a.nnz / kAxesGroups));
   const dim3 grid((unsigned)(((int64_t)r.a.nnz + r.tokens - 1) / r.tokens),
                   (unsigned)((r.a.d / 16 + kAxesFreqs / 8 - 1) / (kAxesFreqs / 8)));
   auto* fn = bf16 ? (interleave ? pick_rope_axes<true, true>(append, fp8)
