@@ -295,6 +295,7 @@ PyObject* decode_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!o.get(a[11], a[12], return_lse, *q, bsz, hq, d)) return general();
   void* stream;
   if (!raw_stream(q->device(), &stream)) return nullptr;
+  const c10::DeviceGuard guard(q->device());
   const void* qp = q->data_ptr();
   const void* kp = append ? k->data_ptr() : nullptr;
   const void* vp = append ? v->data_ptr() : nullptr;
@@ -352,6 +353,7 @@ PyObject* prefill_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!o.get(a[13], a[14], return_lse, *q, q->size(0), hq, d)) return general();
   void* stream;
   if (!raw_stream(q->device(), &stream)) return nullptr;
+  const c10::DeviceGuard guard(q->device());
   const void* qp = q->data_ptr();
   void* pp = pool.ptr();
   void* op = o.out.data_ptr();
@@ -490,6 +492,7 @@ PyObject* axes_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !std::isfinite(rope_theta))
     return general();
   if (!raw_stream(dev, &x.stream)) return nullptr;
+  const c10::DeviceGuard guard(dev);
   void *qp = q->data_ptr(), *kp = x.k->data_ptr(), *pp = x.pool.ptr();
   const void* vp = x.v->data_ptr();
   const auto* ap = static_cast<const int32_t*>(axes->data_ptr());

@@ -591,7 +591,7 @@ static int check_pool(const char* who, const void* kv_pool, int32_t dtype, int32
   if (!esz)
     return set_error(PAGEDATTN_ERR_UNSUPPORTED, "%s: pool dtype %d not supported", who, dtype);
   if (num_layers <= 0 || num_pages < 0 || hkv <= 0 || d <= 0 || (d * esz) % 16 ||
-      (int64_t)2 * hkv * kPage * d * esz > INT32_MAX / 2)
+      (int64_t)hkv * d > INT32_MAX / 2 / (2 * kPage * esz))
     return set_error(PAGEDATTN_ERR_INVALID,
                      "%s: bad shape layers=%d pages=%d hkv=%d d=%d (rows must be a multiple of "
                      "16 bytes)",
@@ -620,8 +620,10 @@ static int check_tables(const char* who, const int32_t* tables, int64_t stride, 
     return set_error(PAGEDATTN_ERR_INVALID,
                      "%s: bad sizes batch=%d max_pages=%d stride=%lld pages=%d", who, batch,
                      max_pages, (long long)stride, num_pages);
-  if (batch > 65535)
-    return set_error(PAGEDATTN_ERR_UNSUPPORTED, "%s: batch_size %d above 65535", who, batch);
+  if (batch > 65535 || (int64_t)batch * ((int64_t)max_pages + 1) > INT32_MAX)
+    return set_error(PAGEDATTN_ERR_UNSUPPORTED,
+                     "%s: batch_size %d above 65535, or with %d pages a row past 2^31 - 1 entries",
+                     who, batch, max_pages);
   if (batch > 0 && max_pages > 0 && !tables)
     return set_error(PAGEDATTN_ERR_INVALID, "%s: null block_tables", who);
   if (num_pages > 0 && !refs)

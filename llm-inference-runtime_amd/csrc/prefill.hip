@@ -187,7 +187,6 @@ __device__ __forceinline__ int fetch_page_ids(const PrefillParams& p,
   return id;
 }
 
-
 // Buffer resource of the K (V = false) or V block of tile page j, sized to
 // its valid tokens: absent pages and slots past last_page_len read as zero.
 template <int D, bool BF16, bool FP8, int RB, bool V, bool WINDOW>

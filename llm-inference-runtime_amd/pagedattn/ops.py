@@ -135,8 +135,9 @@ def _scratch(plan: "_Plan", q: torch.Tensor) -> torch.Tensor | None:
 def _run_plan(entry: str, fn: str, scratch: torch.Tensor | None, device: torch.device,
               *args) -> None:
     """Entry point `fn` with its scratch and stream arguments; errors name `entry`."""
-    rc = getattr(_lib.lib(), fn)(*args, ptr(scratch), 0 if scratch is None else scratch.numel(),
-                                 _stream(device))
+    with torch.cuda.device(device):
+        rc = getattr(_lib.lib(), fn)(*args, ptr(scratch),
+                                     0 if scratch is None else scratch.numel(), _stream(device))
     if rc != 0:
         _lib.raise_status(entry, rc)
 
@@ -538,7 +539,8 @@ def reserve_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, kv_lens: to
     new_lens[b] tokens counted already, as in build_paged_metadata; None: one
     each) and ref_counts [num_pages] are int32 device tensors; tables and counts
     are updated in place.  Every slot that the new tokens open gets a free
-    page (count 0 -> 1), the lowest ids first, in row and slot order.  A
+    page (count 0 -> 1), the lowest ids first, in row and slot order; what the
+    slot named before is not released.  A
     partial page that the tokens continue while others hold it is forked
     (todo.md:17-19): a free page takes its rows in every layer of kv_pool [L, P,
     2, Hkv, 16, D] (and of kv_scales for an e4m3 pool) and its place in the
@@ -975,7 +977,9 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
 
         window_left = w >= 0: every sequence's query, its newest token, sees the
         w tokens before it and itself, and the first num_sink_tokens tokens.
-        Pages it does not see are not read (their entries may be -1)."""
+        Pages it does not see are not read (their entries may be -1).  The ids of
+        those it sees are copied: by plan() here (a step's ids must be in place by
+        then), of device plans by update_plan() or each run."""
         _unsupported_options(pos_encoding_mode, logits_soft_cap)
         window = _window(window_left, num_sink_tokens)
         if page_size != PAGE_SIZE:
@@ -1001,9 +1005,9 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
             raise ValueError(f"indices has {indices.numel()} entries, indptr needs {n_ind}")
         self._q_dtype = _dtype_of(data_type if data_type is not None else q_data_type)
         self._kv_dtype = _dtype_of(kv_data_type) if kv_data_type is not None else None
-        call("pagedattn_decode_plan_window", self._plan.handle, ptr(indptr_h), ptr(last_h), bsz,
-             int(num_qo_heads), int(num_kv_heads), int(head_dim), int(page_size),
-             int(split_pages), *window, ptr(self._ws), self._ws_bytes, _stream(device))
+        _on(device, "pagedattn_decode_plan_window", self._plan.handle, ptr(indptr_h), ptr(last_h),
+            bsz, int(num_qo_heads), int(num_kv_heads), int(head_dim), int(page_size),
+            int(split_pages), *window, ptr(self._ws), self._ws_bytes)
         self._indptr = _i32(indptr, device)
         self._indices = _i32(indices, device)
         self._last = _i32(last_page_len, device)
@@ -1039,10 +1043,10 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
         self._planned = True
 
     def _make_lists(self) -> None:
-        call("pagedattn_decode_window_metadata", ptr(self._indptr), ptr(self._indices),
-             self._indices.numel(), ptr(self._last), self._bsz, self._window_left, self._sinks,
-             ptr(self._seen_indptr), ptr(self._seen_indices), self._seen_indices.numel(),
-             ptr(self._holes), _stream(self._indptr.device))
+        _on(self._indptr.device, "pagedattn_decode_window_metadata", ptr(self._indptr),
+            ptr(self._indices), self._indices.numel(), ptr(self._last), self._bsz,
+            self._window_left, self._sinks, ptr(self._seen_indptr), ptr(self._seen_indices),
+            self._seen_indices.numel(), ptr(self._holes))
 
     def _plan_device(self, indptr, indices, last_page_len, num_qo_heads, num_kv_heads,
                      head_dim, page_size, q_data_type, kv_data_type, data_type, sm_scale):
@@ -1097,9 +1101,9 @@ class BatchDecodeWithPagedKVCacheWrapper(_WrapperBase):
             self._make_lists()
             self._lists_made = True
         if kind == "device_shared":
-            call("pagedattn_decode_plan_device_update", self._plan.handle,
-                 ptr(self._indptr if self._holes is None else self._seen_indptr),
-                 ptr(self._last), _stream(self._indptr.device))
+            _on(self._indptr.device, "pagedattn_decode_plan_device_update", self._plan.handle,
+                ptr(self._indptr if self._holes is None else self._seen_indptr),
+                ptr(self._last))
 
     @property
     def plan_kind(self) -> str | None:
@@ -1289,9 +1293,9 @@ class BatchPrefillWithPagedKVCacheWrapper(_WrapperBase):
             raise ValueError(
                 f"paged_kv_indices has {paged_kv_indices.numel()} entries, indptr needs {n_ind}")
         self._q_dtype = _dtype_of(q_data_type)
-        call("pagedattn_prefill_plan_window", self._plan.handle, ptr(qo_h), ptr(indptr_h),
-             ptr(last_h), bsz, int(num_qo_heads), int(num_kv_heads), int(head_dim_qk),
-             int(page_size), *window, ptr(self._ws), self._ws_bytes, _stream(device))
+        _on(device, "pagedattn_prefill_plan_window", self._plan.handle, ptr(qo_h), ptr(indptr_h),
+            ptr(last_h), bsz, int(num_qo_heads), int(num_kv_heads), int(head_dim_qk),
+            int(page_size), *window, ptr(self._ws), self._ws_bytes)
         self._qo_rows = int(qo_h[-1]) if bsz else 0
 
     begin_forward = plan

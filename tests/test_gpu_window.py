@@ -547,3 +547,33 @@ def test_decode_by_the_general_path(gpu, kind, request):
         fused = w.run(q, p, append_key=k, append_value=v, rope=(1.0, 1e4))
         got.append((out, lse, fused, p.view(torch.int16)))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_prefill_of_scales_not_finite(gpu):
+    """The scale of a page that some rows of a tile see is an infinity, of another NaN: the rows
+    that see neither are as if the pages were not there."""
+    heads, dtype, window, sinks = HEADS[1], torch.bfloat16, 25, 0
+    meta, pool, scales, q = make(gpu, [0], [150], heads, dtype, True, window, sinks, seed=9)
+    table = meta.kv_indices
+    scales[int(table[3])] = math.inf  # tokens 48 to 63
+    scales[int(table[6])] = math.nan  # tokens 96 to 111
+    clear = [r for r in range(150) if not (48 <= r <= 63 + window or 96 <= r <= 111 + window)]
+    assert len(clear) > 20
+    w = plan_prefill(gpu, meta, heads, dtype, window, sinks, False)
+    out, lse = w.run(q, pool, kv_scales=scales, return_lse=True)
+    check(out, lse, reference(meta, pool, scales, q, window, sinks, b_rows=set(clear)), clear)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+@pytest.mark.parametrize("kind", ["host", "device"])
+@pytest.mark.parametrize("way", ["extension", "general"])
+def test_decode_on_a_device_that_is_not_current(gpu, kind, way, request):
+    if way == "general":
+        request.getfixturevalue("general")
+    heads, dtype, window, sinks = HEADS[0], torch.float16, 50, 4
+    other = torch.device("cuda", 1)
+    meta, pool, scales, q = make(other, [99, 300], [1, 1], heads, dtype, False, window, sinks,
+                                 seed=3)
+    assert torch.cuda.current_device() == 0
+    w = plan_decode(other, meta, heads, dtype, window, sinks, kind)
+    check(*w.run(q, pool, return_lse=True), reference(meta, pool, scales, q, window, sinks))

@@ -100,10 +100,12 @@ BAD_POOLS = [({"page": 8}, UNSUPPORTED, "page_size"), ({"dtype": _lib.F32}, UNSU
              ({"layers": 0}, INVALID, "shape"), ({"hkv": 0}, INVALID, "shape"),
              ({"d": 4}, INVALID, "16 bytes"), ({"d": 8, "dtype": _lib.E4M3}, INVALID, "16 bytes"),
              ({"dtype": _lib.E4M3}, INVALID, "kv_scales"), ({"pool": None}, INVALID, "pool"),
-             ({"pool": A + 8}, INVALID, "pool"), ({"pages": -1}, INVALID, "shape")]
+             ({"pool": A + 8}, INVALID, "pool"), ({"pages": -1}, INVALID, "shape"),
+             ({"hkv": 1 << 30, "d": 1 << 30}, INVALID, "shape")]
 BAD_TABLES = [({"tables": None}, INVALID, "null block_tables"), ({"refs": None}, INVALID, "ref"),
               ({"stride": 3}, INVALID, "bad sizes"), ({"b": -1}, INVALID, "bad sizes"),
-              ({"width": -1}, INVALID, "bad sizes"), ({"b": 65536}, UNSUPPORTED, "65535")]
+              ({"width": -1}, INVALID, "bad sizes"), ({"b": 65536}, UNSUPPORTED, "65535"),
+              ({"b": 65535, "width": 1 << 15, "stride": 1 << 15}, UNSUPPORTED, "entries")]
 BAD_SCRATCH = [({"scratch": None}, INVALID, "scratch"), ({"scratch": A + 64}, INVALID, "scratch"),
                ({"size": 100}, WORKSPACE, "scratch")]
 
