@@ -145,6 +145,26 @@ inline __host__ __device__ int window_page(const WindowTiles& w, int listed) {
   return listed < w.sink_pages ? listed : listed + w.shift;
 }
 
+// Place in a windowed plan's list of the tile that is rank `rank` of n, longest first,
+// where `slots` of them run at once per KV head.  Under a window most tiles are
+// equally long: workgroups that start together end together, round after round,
+// and the bytes of all their Q and output rows move while no matrix core works. So
+// every other one of the `slots` shortest goes ahead, which sets the first round's
+// ends apart (the others still fill the last one).  Of more than two rounds, 32/8
+// heads, D = 128, us in the order of length and in this one: prompts of 7923 and 6653
+// tokens, window 1023, 300 and 284 (e4m3 320 and 310); 4 of 3000, 511, 163 and 148;
+// 20 of 700, 255, 141 and 128; 16 of 300, 127, 41 and 38; 2 of 8000, 4095, 768 and
+// 768.  32/4, D = 64, two workgroups a CU, gains 0 to 6 %.  Of fewer rounds the last
+// one loses what the first gains (2500 tokens, 1023, 53 and 56), and the order stays.
+inline __host__ __device__ int prefill_place(int rank, int n, int slots) {
+  if (n <= 2 * (int64_t)slots) return rank;
+  const int k = n - 1 - rank;             // from the list's end
+  const int ahead = (slots + 1) / 2;      // those with an even k below `slots`
+  if (k >= slots) return ahead + rank;
+  if (k % 2 == 0) return ahead - 1 - k / 2;
+  return ahead + rank - (ahead - (k + 1) / 2);
+}
+
 // The pages of a decode step's sequence of `npages` pages, the last holding
 // `last` tokens, that its newest token sees: `npages` listed ones, those of the
 // sinks and those from the window's start on, with a hole [hole_lo, hole_hi) of
@@ -229,6 +249,8 @@ struct pagedattn_plan {
   int q_tile = 0;
   // prefill: the window's tokens before a token (-1: no window), and the sinks
   int window_left = -1, sinks = 0;
+  // prefill: windowed tiles of a KV head that run at once (prefill_place)
+  int round_tiles = 0;
   // prefill: tiles of at most half a workgroup's rows run as KV-head pairs
   // (device plans apply it at run time; host plans flag their items)
   bool prefill_pair = false;

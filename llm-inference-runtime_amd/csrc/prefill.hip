@@ -1070,7 +1070,7 @@ struct PrefillPlanArgs {
   PrefillPiece* pieces;
   PrefillMerge* merges;
   int32_t* n_merge;
-  int32_t window_left, sinks;
+  int32_t window_left, sinks, round_tiles;
 };
 
 constexpr int kPrefillPlanThreads = 1024;
@@ -1223,9 +1223,10 @@ __global__ void __launch_bounds__(kPrefillPlanThreads) prefill_plan_kernel(Prefi
     if (t < n_tiles) {
       // paired tiles alternate between the even and the odd head of a head
       // pair by list position, so both XCDs of the pair share them
-      if (it.slot > 0) it.slot = 1 + (rank & 1);
-      a.items[rank] = it;
-      if (len == 0) put_piece(rank, it);
+      const int at = a.window_left >= 0 ? prefill_place(rank, n_tiles, a.round_tiles) : rank;
+      if (it.slot > 0) it.slot = 1 + (at & 1);
+      a.items[at] = it;
+      if (len == 0) put_piece(at, it);
     }
   } else {
     for (int i = t; i < n_tiles; i += kPrefillPlanThreads) {
@@ -1260,7 +1261,7 @@ static int launch_prefill_plan(const pagedattn_plan* plan, const int32_t* qo_ind
                     plan->scratch_bytes ? plan->n_slots : 0, plan->n_pieces,
                     static_cast<PrefillPiece*>(plan->pieces_dev),
                     static_cast<PrefillMerge*>(plan->merge_dev), plan->n_merge_dev,
-                    plan->window_left, plan->sinks};
+                    plan->window_left, plan->sinks, plan->round_tiles};
   hipLaunchKernelGGL(prefill_plan_kernel, dim3(1), dim3(kPrefillPlanThreads), 0,
                      (hipStream_t)stream, a);
   return check_launch(who);

@@ -235,6 +235,11 @@ int pagedattn_prefill_plan_window(pagedattn_plan* plan, const int32_t* qo_indptr
                 sizeof(PrefillMerge) * merges.size());
   }
   auto* dst = reinterpret_cast<PrefillItem*>(hb);
+  if (window_left >= 0) {
+    const std::vector<int> by_length = order;
+    const int n = (int)order.size();
+    for (int i = 0; i < n; ++i) order[prefill_place(i, n, (int)slots)] = by_length[i];
+  }
   // paired tiles alternate between the even and the odd head of each pair in
   // list order, so the two XCDs that hold a head pair's workgroups share them
   int n_paired = 0;
@@ -317,6 +322,7 @@ int pagedattn_prefill_plan_device_window(pagedattn_plan* plan, int32_t batch_siz
   plan->q_tile = q_tile;
   plan->window_left = window_left;
   plan->sinks = sinks;
+  plan->round_tiles = (int)prefill_split_slots(num_kv_heads);
   plan->total_qo = max_qo_tokens;
   plan->items_dev = static_cast<char*>(workspace) + kWsHeader;
   // the plan kernel may cut tiles, on the host plan's rule (the tiles are known

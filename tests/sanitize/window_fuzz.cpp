@@ -110,6 +110,18 @@ const char* walk_of(const Window& w) {
   return nullptr;
 }
 
+// The list places of a plan's tiles are a permutation.
+const char* places_of() {
+  const int n = (int)uni(0, 300), slots = (int)uni(1, 120);
+  std::vector<bool> taken(n, false);
+  for (int i = 0; i < n; ++i) {
+    const int at = pa::prefill_place(i, n, slots);
+    if (at < 0 || at >= n || taken[at]) return "list places";
+    taken[at] = true;
+  }
+  return nullptr;
+}
+
 // Extreme sizes: nothing overflows, and the walk stays inside the sequence.
 const char* extremes_of(const Window& w) {
   const int64_t kv_end = INT_MAX - uni(0, 100);
@@ -217,6 +229,23 @@ const char* dealt(const pagedattn_plan* p, const Meta& m, const Window& w) {
   return nullptr;
 }
 
+// A windowed prefill plan's list holds every query token once.
+const char* tiled(const pagedattn_plan* p, const Meta& m) {
+  std::vector<pa::PrefillItem> items;
+  if (!inside(p->items_dev, p->n_items, &items)) return "tiles outside the workspace";
+  std::sort(items.begin(), items.end(), [](auto& x, auto& y) { return x.q_lo < y.q_lo; });
+  std::vector<int> at(m.batch, 0);
+  for (auto& i : items) {
+    if (i.b < 0 || i.b >= m.batch || i.q_lo != at[i.b] || i.q_hi <= i.q_lo ||
+        i.q_hi - i.q_lo > p->q_tile)
+      return "query tokens not covered once";
+    at[i.b] = i.q_hi;
+  }
+  for (int b = 0; b < m.batch; ++b)
+    if (at[b] != m.qo[b + 1] - m.qo[b]) return "query tokens not covered";
+  return nullptr;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -230,6 +259,7 @@ int main(int argc, char** argv) {
     const Window w = make_window();
     const char* wrong = lists_of(w);
     if (!wrong) wrong = walk_of(w);
+    if (!wrong) wrong = places_of();
     if (!wrong) wrong = extremes_of(w);
     const Meta m = make_meta();
     const bool bad_window = coin(0.1);
@@ -252,7 +282,7 @@ int main(int argc, char** argv) {
       wrong = decode ? "decode plan's status" : "prefill plan's status";
     if (!wrong && rc == PAGEDATTN_OK) {
       ++plans;
-      if (decode) wrong = dealt(plan, m, w);
+      wrong = decode ? dealt(plan, m, w) : tiled(plan, m);
     }
     pagedattn_plan_destroy(plan);
     if (wrong) {
