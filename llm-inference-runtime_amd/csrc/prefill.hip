@@ -843,20 +843,61 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
           continue;
         }
       }
-      if (!rvalid[rb]) continue;
+      const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
       const int row = 32 * (RB * wave + rb) + col;
       const int qi = q_lo + row / g;
       const int head = h * g + row % g;
-      const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
-      uint16_t* orow = p.out + ((int64_t)(qo_start + qi) * p.hq + head) * D;
+      if constexpr (WINDOW) {
+        // Stores of 64 bytes of a row in place of 16: the halves of a 16-byte chunk to
+        // one lane, then chunks 2 and 3 of a row to the lanes of the row 16 below, whose
+        // chunks 0 and 1 come to this one's.  Lanes of rows 0 to 15 and 16 to 31 then
+        // hold 64 bytes of rows 0 to 15 in x[0] and of rows 16 to 31 in x[1].
+        uint16_t* to[2];
+        bool on[2];
 #pragma unroll
-      for (int dt = 0; dt < C::DT; ++dt) {
+        for (int k = 0; k < 2; ++k) {
+          const int r = 32 * (RB * wave + rb) + 16 * k + (lane & 15);
+          on[k] = q_lo + r / g < q_hi;
+          to[k] = p.out + ((int64_t)(qo_start + q_lo + r / g) * p.hq + h * g + r % g) * D +
+                  8 * (2 * ((lane >> 4) & 1) + half);
+        }
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          u32x2 w;
-          w[0] = pack2_16<BF16>(o[rb][dt][4 * i4] * inv, o[rb][dt][4 * i4 + 1] * inv);
-          w[1] = pack2_16<BF16>(o[rb][dt][4 * i4 + 2] * inv, o[rb][dt][4 * i4 + 3] * inv);
-          *reinterpret_cast<u32x2*>(orow + 32 * dt + 8 * i4 + 4 * half) = w;
+        for (int dt = 0; dt < C::DT; ++dt) {
+          u32x4 x[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const int r = 8 * j + 2 * w;
+              const auto c = __builtin_amdgcn_permlane32_swap(
+                  pack2_16<BF16>(o[rb][dt][r] * inv, o[rb][dt][r + 1] * inv),
+                  pack2_16<BF16>(o[rb][dt][r + 4] * inv, o[rb][dt][r + 5] * inv), false, false);
+              x[j][w] = c[0];
+              x[j][2 + w] = c[1];
+            }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const auto c = __builtin_amdgcn_permlane16_swap(x[0][w], x[1][w], false, false);
+            x[0][w] = c[0];
+            x[1][w] = c[1];
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (on[k]) *reinterpret_cast<u32x4*>(to[k] + 32 * dt) = x[k];
+        }
+      }
+      if (!rvalid[rb]) continue;
+      if constexpr (!WINDOW) {
+        uint16_t* orow = p.out + ((int64_t)(qo_start + qi) * p.hq + head) * D;
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            u32x2 w;
+            w[0] = pack2_16<BF16>(o[rb][dt][4 * i4] * inv, o[rb][dt][4 * i4 + 1] * inv);
+            w[1] = pack2_16<BF16>(o[rb][dt][4 * i4 + 2] * inv, o[rb][dt][4 * i4 + 3] * inv);
+            *reinterpret_cast<u32x2*>(orow + 32 * dt + 8 * i4 + 4 * half) = w;
+          }
         }
       }
       if (p.lse && half == 0)
