@@ -429,6 +429,10 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
   if constexpr (WINDOW)
     wt = window_tiles(kv_end, (int64_t)diag + q_lo, p.window_left, p.sinks);
   const int n_tiles = WINDOW ? wt.total : (kv_end + BN - 1) / BN;
+  // the first row's last visible token, and the last row's first one past the sinks
+  const int lim_first = p.causal ? min(diag + q_lo, kv_len - 1) : kv_len - 1;
+  const int pos_last = max(0, diag + q_hi - 1);
+  const int wlo_last = pos_last - min(pos_last, p.window_left);
   // the KV tiles [t_lo, t_hi) of this workgroup: all of them, or piece k of n
   int t_lo = 0, t_hi = n_tiles, slot = -1;
   if constexpr (SPLIT) {
@@ -577,21 +581,31 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
               if (32 * mt + 8 * (i >> 2) + (i & 3) > rel) s[rb][mt][i] = -INFINITY;
         }
         if constexpr (MASK && WINDOW) {
-          // page by page: visible iff offset <= rel, and >= rel_lo or < rel_sink
+          // page by page: visible iff offset <= rel, and >= rel_lo or < rel_sink.
+          // Sides on which all rows of the tile see the whole page are passed over
+          // (20 prompts of 700 tokens, window 255: 109 -> 106 us), but without branches
+          // at D = 64: they would spill 34 VGPRs past the 128 that leave the CU its
+          // second workgroup.
+          constexpr bool BRANCH = D != 64 || FP8;
 #pragma unroll
           for (int pg = 0; pg < 4; ++pg) {
-            const int at = kPage * window_page(wt, 4 * t + pg) + 4 * half;
-            const int rel = lim[rb] - at;
-            const int rel_lo = wlo[rb] - at;
-            const int rel_sink = p.sinks - at;
+            const int at = kPage * window_page(wt, 4 * t + pg);
+            const int rel = lim[rb] - at - 4 * half;
+            const int rel_lo = wlo[rb] - at - 4 * half;
+            const int rel_sink = p.sinks - at - 4 * half;
+            auto hide = [&](auto hidden) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int off = 8 * (i >> 2) + (i & 3);
-              // without branches: 122 VGPRs at D = 64, where more than 128 would
-              // cost the CU's second workgroup (160 with them)
-              const bool hidden = (off > rel) | ((off < rel_lo) & (off >= rel_sink));
-              const float x = s[rb][pg >> 1][8 * (pg & 1) + i];
-              s[rb][pg >> 1][8 * (pg & 1) + i] = hidden ? -INFINITY : x;
+              for (int i = 0; i < 8; ++i) {
+                const float x = s[rb][pg >> 1][8 * (pg & 1) + i];
+                s[rb][pg >> 1][8 * (pg & 1) + i] = hidden(8 * (i >> 2) + (i & 3)) ? -INFINITY : x;
+              }
+            };
+            if constexpr (BRANCH) {
+              if (at + kPage - 1 > lim_first) hide([&](int off) { return off > rel; });
+              if (at < wlo_last && at > p.sinks - kPage)
+                hide([&](int off) { return (off < rel_lo) & (off >= rel_sink); });
+            } else {
+              hide([&](int off) { return (off > rel) | ((off < rel_lo) & (off >= rel_sink)); });
             }
           }
         }
@@ -717,9 +731,8 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
     // masked too, [t_lo, n_edge), unless no row's window leaves anything out.
     int n_edge = t_lo, n_clean = 0;
     if constexpr (WINDOW) {
-      const int last_lo = max(0, diag + q_hi - 1) - min(max(0, diag + q_hi - 1), p.window_left);
-      if (last_lo > p.sinks) {
-        const int pages = max(wt.sink_pages, (last_lo + kPage - 1) / kPage - wt.shift);
+      if (wlo_last > p.sinks) {
+        const int pages = max(wt.sink_pages, (wlo_last + kPage - 1) / kPage - wt.shift);
         n_edge = max(t_lo, min(t_hi, (pages + 3) / 4));
       }
       n_clean = min(t_hi, max(n_edge, (clean_end / kPage - wt.shift) / 4));
@@ -883,7 +896,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            if (on[k]) *reinterpret_cast<u32x4*>(to[k] + 32 * dt) = x[k];
+            if (on[k]) __builtin_nontemporal_store(x[k], reinterpret_cast<u32x4*>(to[k] + 32 * dt));
         }
       }
       if (!rvalid[rb]) continue;
