@@ -304,7 +304,12 @@ __device__ __forceinline__ void copy_pages(const CopyArgs& c, int64_t wg, int64_
     }
 #pragma unroll
     for (int k = 0; k < kCopyLoads; ++k)
-      if (on[k]) *reinterpret_cast<u32x4*>(d + at[k]) = x[k];
+      if (on[k]) {
+        // a compacted pool is past the caches (a streamed store: 263 -> 252 us); a
+        // fork's page is the next one written and read
+        if constexpr (ROWS) *reinterpret_cast<u32x4*>(d + at[k]) = x[k];
+        else __builtin_nontemporal_store(x[k], reinterpret_cast<u32x4*>(d + at[k]));
+      }
     if (c.scales && part == 0)
       for (int j = (int)threadIdx.x; j < c.blocks; j += kPageThreads)
         c.scales[to * c.blocks + j] = c.scales[from * c.blocks + j];

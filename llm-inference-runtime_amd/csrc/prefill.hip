@@ -864,7 +864,10 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
         // Stores of 64 bytes of a row in place of 16: the halves of a 16-byte chunk to
         // one lane, then chunks 2 and 3 of a row to the lanes of the row 16 below, whose
         // chunks 0 and 1 come to this one's.  Lanes of rows 0 to 15 and 16 to 31 then
-        // hold 64 bytes of rows 0 to 15 in x[0] and of rows 16 to 31 in x[1].
+        // hold 64 bytes of rows 0 to 15 in x[0] and of rows 16 to 31 in x[1].  20 prompts
+        // of 700 tokens, window 255: 128 -> 118 us.  And streamed past the L2: 14 000
+        // tokens 127 -> 118 us alone, 507 -> 502 with a 4096 x 4096 product of the
+        // output after it.
         uint16_t* to[2];
         bool on[2];
 #pragma unroll
