@@ -861,45 +861,70 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, WINDOW && D == 64 && !FP8 
       const int qi = q_lo + row / g;
       const int head = h * g + row % g;
       if constexpr (WINDOW) {
-        // Stores of 64 bytes of a row in place of 16: the halves of a 16-byte chunk to
-        // one lane, then chunks 2 and 3 of a row to the lanes of the row 16 below, whose
-        // chunks 0 and 1 come to this one's.  Lanes of rows 0 to 15 and 16 to 31 then
-        // hold 64 bytes of rows 0 to 15 in x[0] and of rows 16 to 31 in x[1].  20 prompts
-        // of 700 tokens, window 255: 128 -> 118 us.  And streamed past the L2: 14 000
-        // tokens 127 -> 118 us alone, 507 -> 502 with a 4096 x 4096 product of the
-        // output after it.
-        uint16_t* to[2];
-        bool on[2];
+        // Stores of whole 128-byte lines in place of 16 bytes of a row: the halves of
+        // a 16-byte chunk to one lane, then chunks 2 and 3 of a row's tile to the lanes
+        // of the row 16 below, whose chunks 0 and 1 come to this one's, and the second
+        // of two tiles to the lanes of the row 8 below.  x[m][k] then holds a line of
+        // rows 16 k + 8 m to 16 k + 8 m + 7.  14 000 tokens, window 255: 135 us with 16
+        // bytes, 127 with 64, 118 with 64 streamed past the L2, where half lines cost
+        // 42 % more HBM bytes written, 116 with whole lines, which cost none; and 502
+        // and 497 us where a 4096 x 4096 product of the output follows (64 bytes,
+        // and these).
+        uint16_t* to[2][2];
+        bool on[2][2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int r = 32 * (RB * wave + rb) + 16 * k + (lane & 15);
-          on[k] = q_lo + r / g < q_hi;
-          to[k] = p.out + ((int64_t)(qo_start + q_lo + r / g) * p.hq + h * g + r % g) * D +
-                  8 * (2 * ((lane >> 4) & 1) + half);
-        }
+        for (int m_ = 0; m_ < 2; ++m_)
 #pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt) {
-          u32x4 x[2];
+          for (int k = 0; k < 2; ++k) {
+            const int r = 32 * (RB * wave + rb) + 16 * k + 8 * m_ + (lane & 7);
+            on[m_][k] = q_lo + r / g < q_hi;
+            to[m_][k] = p.out +
+                        ((int64_t)(qo_start + q_lo + r / g) * p.hq + h * g + r % g) * D +
+                        32 * ((lane >> 3) & 1) + 8 * (2 * ((lane >> 4) & 1) + half);
+          }
+        const bool upper = lane & 8;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+        for (int dp = 0; dp < C::DT; dp += 2) {
+          u32x4 x[2][2];
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const int r = 8 * j + 2 * w;
-              const auto c = __builtin_amdgcn_permlane32_swap(
-                  pack2_16<BF16>(o[rb][dt][r] * inv, o[rb][dt][r + 1] * inv),
-                  pack2_16<BF16>(o[rb][dt][r + 4] * inv, o[rb][dt][r + 5] * inv), false, false);
-              x[j][w] = c[0];
-              x[j][2 + w] = c[1];
+          for (int m_ = 0; m_ < 2; ++m_) {
+            const f32x16& y = o[rb][dp + m_];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const int r = 8 * j + 2 * w;
+                const auto c = __builtin_amdgcn_permlane32_swap(
+                    pack2_16<BF16>(y[r] * inv, y[r + 1] * inv),
+                    pack2_16<BF16>(y[r + 4] * inv, y[r + 5] * inv), false, false);
+                x[m_][j][w] = c[0];
+                x[m_][j][2 + w] = c[1];
+              }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const auto c =
+                  __builtin_amdgcn_permlane16_swap(x[m_][0][w], x[m_][1][w], false, false);
+              x[m_][0][w] = c[0];
+              x[m_][1][w] = c[1];
             }
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const auto c = __builtin_amdgcn_permlane16_swap(x[0][w], x[1][w], false, false);
-            x[0][w] = c[0];
-            x[1][w] = c[1];
           }
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (on[k]) __builtin_nontemporal_store(x[k], reinterpret_cast<u32x4*>(to[k] + 32 * dt));
+          for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              // lane ^ 8: a rotation of 16 lanes by 8
+              const uint32_t out = upper ? x[0][k][w] : x[1][k][w];
+              const uint32_t in = (uint32_t)__builtin_amdgcn_update_dpp(
+                  0, (int)out, 0x128, 0xf, 0xf, false);
+              if (upper) x[0][k][w] = in;
+              else x[1][k][w] = in;
+            }
+#pragma unroll
+            for (int m_ = 0; m_ < 2; ++m_)
+              if (on[m_][k])
+                __builtin_nontemporal_store(x[m_][k],
+                                            reinterpret_cast<u32x4*>(to[m_][k] + 32 * dp));
+          }
         }
       }
       if (!rvalid[rb]) continue;
