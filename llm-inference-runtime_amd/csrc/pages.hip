@@ -199,17 +199,75 @@ __global__ void __launch_bounds__(kPageThreads) reserve_count_kernel(ReserveArgs
   }
 }
 
+// What reserve_count_kernel counts for sequence threadIdx.x of up to kPageThreads,
+// by a whole workgroup; *ok: the sequence is not skipped.
+__device__ __forceinline__ int own_need(const ReserveArgs& a, int* part_page, bool* ok) {
+  const int b = (int)threadIdx.x;
+  RowStep r{true, 0, 0, -1, 0};
+  int page = -1, held = 0;
+  if (b < a.batch) {
+    r = row_step(a, b);
+    if (r.ok && r.part >= 0) {
+      page = a.tables[b * a.stride + r.part];
+      if (page >= 0 && page < a.num_pages) held = a.refs[page];
+    }
+  }
+  part_page[b] = page;
+  __syncthreads();
+  *ok = r.ok && (r.part < 0 || held > 0);
+  if (!*ok) return 0;
+  bool fork = false;
+  if (held > 1) {
+    int earlier = 0;
+    for (int i = 0; i < b; ++i) earlier += part_page[i] == page;
+    fork = held - earlier > 1;
+  }
+  return (r.last - r.first) + (fork ? 1 + kForkBit : 0);
+}
+
+// COUNTS: the counts come from reserve_count_kernel.  Up to kPageThreads sequences
+// over a pool of up to kOwnBlocks blocks are counted by every workgroup itself,
+// which saves a launch.
+constexpr int kOwnBlocks = 4;
+
 // Workgroups [0, n_blocks): the free pages of a block at their ranks, as far as
 // they are wanted.  The last: the sequences' first ranks, the forks, and whether
 // the pages suffice.
+template <bool COUNTS>
 __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs a) {
   __shared__ int red[kPageThreads / kWave];
-  if ((int)blockIdx.x == a.n_blocks) {
-    const int total_free = array_sum(a.free_cnt, a.n_blocks, red);
+  __shared__ int part_page[COUNTS ? 1 : kPageThreads];
+  const int blk = (int)blockIdx.x;
+  const bool last = blk == a.n_blocks;
+  // the block's pages are on their way while the counts are summed
+  Held held;
+  if (!last) held.load(a.refs, blk, a.num_pages, true);
+  // free pages before the block (the last workgroup: all), and those wanted
+  int before, wanted, own = 0;
+  if constexpr (COUNTS) {
+    before = array_sum(a.free_cnt, blk, red);
+  } else {
+    int taken = 0;  // the wave's share of the blocks'
+#pragma unroll
+    for (int i = 0; i < kOwnBlocks; ++i)
+      if (i < blk) {
+        Held other;
+        other.load(a.refs, i, a.num_pages, true);
+        taken += other.count();
+      }
+    int unused;
+    before = blk * kPagesPerBlock - waves_sum(taken, red, &unused);
+    bool ok;
+    own = own_need(a, part_page, &ok);
+    if (last && !ok && a.err) atomicAdd(a.err, 1);
+  }
+  if (last) {
     int run = 0, forks = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
       const int b = b0 + (int)threadIdx.x;
-      const int need = b < a.batch ? a.need[b] : 0;
+      int need = own;
+      if constexpr (COUNTS) need = b < a.batch ? a.need[b] : 0;
+      else if (b < a.batch) a.need[b] = need;
       const bool fork = need & kForkBit;
       int total, total_forks;
       __syncthreads();
@@ -226,20 +284,19 @@ __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs 
       forks += total_forks;
     }
     if (threadIdx.x == 0) {
-      const int missing = max(run - total_free, 0);
+      const int missing = max(run - before, 0);
       *a.short_of = missing;
       *a.n_forks = missing > 0 ? 0 : forks;
       if (missing > 0 && a.err) atomicAdd(a.err + 1, missing);
     }
     return;
   }
-  // the block's pages are on their way while the counts are summed
-  Held held;
-  held.load(a.refs, (int)blockIdx.x, a.num_pages, true);
-  int wanted = 0;
-  for (int b = (int)threadIdx.x; b < a.batch; b += kPageThreads) wanted += a.need[b] & ~kForkBit;
+  wanted = own & ~kForkBit;
+  if constexpr (COUNTS) {
+    wanted = 0;
+    for (int b = (int)threadIdx.x; b < a.batch; b += kPageThreads) wanted += a.need[b] & ~kForkBit;
+  }
   wanted = block_sum(wanted, red);
-  const int before = array_sum(a.free_cnt, (int)blockIdx.x, red);
   if (before >= wanted) return;  // uniform
   int held_before;
   waves_sum(held.count(), red, &held_before);
@@ -471,8 +528,6 @@ __global__ void __launch_bounds__(kPageThreads) compact_count_kernel(CompactArgs
 
 // COUNTS: the blocks' counts come from compact_count_kernel.  Pools of up to
 // kOwnBlocks blocks are counted by every workgroup itself, which saves a launch.
-constexpr int kOwnBlocks = 4;
-
 template <bool COUNTS>
 __global__ void __launch_bounds__(kPageThreads) compact_rank_kernel(CompactArgs a) {
   __shared__ int red[kPageWaves];
@@ -718,13 +773,17 @@ int pagedattn_reserve_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layer
   a.short_of = a.n_forks + 1;
   a.fresh = at;
   hipStream_t s = (hipStream_t)stream;
-  const unsigned waves = (unsigned)((batch_size + kPageThreads / kWave - 1) / (kPageThreads / kWave));
-  hipLaunchKernelGGL(reserve_count_kernel, dim3((unsigned)a.n_blocks + waves), dim3(kPageThreads),
-                     0, s, a);
-  rc = check_launch(who);
-  if (rc) return rc;
-  hipLaunchKernelGGL(reserve_rank_kernel, dim3((unsigned)a.n_blocks + 1), dim3(kPageThreads), 0, s,
-                     a);
+  const bool counts = a.n_blocks > kOwnBlocks || batch_size > kPageThreads;
+  if (counts) {
+    const unsigned waves =
+        (unsigned)((batch_size + kPageThreads / kWave - 1) / (kPageThreads / kWave));
+    hipLaunchKernelGGL(reserve_count_kernel, dim3((unsigned)a.n_blocks + waves),
+                       dim3(kPageThreads), 0, s, a);
+    rc = check_launch(who);
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(counts ? reserve_rank_kernel<true> : reserve_rank_kernel<false>,
+                     dim3((unsigned)a.n_blocks + 1), dim3(kPageThreads), 0, s, a);
   rc = check_launch(who);
   if (rc) return rc;
   c.count = a.n_forks;

@@ -419,3 +419,31 @@ def test_the_extension_takes_the_plain_form(gpu, path, monkeypatch):
             pagedattn.release_window_pages(x["t"], x["n"], x["r"], x["w"], x["s"],
                                            error_flag=x["err"])
     assert t.tolist() == [[0, -1]] and r.tolist() == [1] + [0] * 8
+
+
+@pytest.mark.parametrize("num_pages", [16384, 16385, 40000])
+@pytest.mark.parametrize("n", [1, 255, 256, 257])
+@pytest.mark.parametrize("short", [False, True])
+def test_reserve_counted_by_every_workgroup_or_ahead(gpu, num_pages, n, short):
+    """Batches and pools on both sides of the sizes that a call counts in a launch of its own:
+    families on one partial page, rows that are skipped, and pools that are nearly full."""
+    rng = np.random.default_rng(num_pages + n + short)
+    lens = rng.integers(1, 300, n)
+    new = rng.integers(0, 40, n)
+    samples = [(b, b // 8 * 8) for b in range(n) if b % 8 and b % 3]
+    for row, of in samples:
+        lens[row] = lens[of]
+    tables, refs = held_tables(rng, num_pages, lens, 24, samples)
+    new[n // 2] = 2000  # past the table
+    wanted = 8 * n if not short else 0
+    others = np.flatnonzero(refs == 0)  # pages of other tables
+    refs[rng.permutation(others)[:max(len(others) - wanted - 1, 0)]] = 3
+    pool, scales = make_pool(gpu, num_pages, POOLS[4])
+    want = Oracle(tables, refs, pool, scales)
+    want.reserve(lens + new, new)
+    t, r, err = i32(tables, gpu), i32(refs, gpu), flags(gpu)
+    pagedattn.reserve_pages(pool, t, i32(lens + new, gpu), i32(new, gpu), r, kv_scales=scales,
+                            error_flag=err)
+    want.check(t, r, pool, scales)
+    assert err.tolist() == [want.rows_bad, want.short] and want.rows_bad == 1
+    assert (want.short > 0) == (short and n > 1)
