@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kPageThreads) reserve_count_kernel(ReserveArgs
   }
 }
 
-// What reserve_count_kernel counts for sequence threadIdx.x of up to kPageThreads,
+// What reserve_count_kernel counts for sequence threadIdx.x of at most kPageThreads,
 // by a whole workgroup; *ok: the sequence is not skipped.
 __device__ __forceinline__ int own_need(const ReserveArgs& a, int* part_page, bool* ok) {
   const int b = (int)threadIdx.x;
@@ -225,10 +225,14 @@ __device__ __forceinline__ int own_need(const ReserveArgs& a, int* part_page, bo
   return (r.last - r.first) + (fork ? 1 + kForkBit : 0);
 }
 
-// COUNTS: the counts come from reserve_count_kernel.  Up to kPageThreads sequences
-// over a pool of up to kOwnBlocks blocks are counted by every workgroup itself,
-// which saves a launch.
-constexpr int kOwnBlocks = 4;
+// COUNTS: the counts come from reserve_count_kernel.  Up to kOwnRows sequences over a
+// pool of up to kReserveBlocks blocks are counted by every workgroup itself, which
+// saves a launch.  Back to back on the GPU, us with and without it: 32 rows over 4000
+// pages 8.1 and 6.2, 128 over 4000 8.4 and 7.5, over 8192 8.6 and 8.2; 256 over 4000
+// 9.0 and 9.3, over 16384 9.5 and 11.5, 32 over 16384 8.5 both.
+constexpr int kOwnRows = 128;
+constexpr int kReserveBlocks = 2;
+static_assert(kOwnRows <= kPageThreads, "a sequence per thread");
 
 // Workgroups [0, n_blocks): the free pages of a block at their ranks, as far as
 // they are wanted.  The last: the sequences' first ranks, the forks, and whether
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kPageThreads) reserve_rank_kernel(ReserveArgs 
   } else {
     int taken = 0;  // the wave's share of the blocks'
 #pragma unroll
-    for (int i = 0; i < kOwnBlocks; ++i)
+    for (int i = 0; i < kReserveBlocks; ++i)
       if (i < blk) {
         Held other;
         other.load(a.refs, i, a.num_pages, true);
@@ -528,6 +532,8 @@ __global__ void __launch_bounds__(kPageThreads) compact_count_kernel(CompactArgs
 
 // COUNTS: the blocks' counts come from compact_count_kernel.  Pools of up to
 // kOwnBlocks blocks are counted by every workgroup itself, which saves a launch.
+constexpr int kOwnBlocks = 4;
+
 template <bool COUNTS>
 __global__ void __launch_bounds__(kPageThreads) compact_rank_kernel(CompactArgs a) {
   __shared__ int red[kPageWaves];
@@ -773,7 +779,7 @@ int pagedattn_reserve_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layer
   a.short_of = a.n_forks + 1;
   a.fresh = at;
   hipStream_t s = (hipStream_t)stream;
-  const bool counts = a.n_blocks > kOwnBlocks || batch_size > kPageThreads;
+  const bool counts = a.n_blocks > kReserveBlocks || batch_size > kOwnRows;
   if (counts) {
     const unsigned waves =
         (unsigned)((batch_size + kPageThreads / kWave - 1) / (kPageThreads / kWave));
