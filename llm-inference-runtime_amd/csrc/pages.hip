@@ -13,8 +13,8 @@
 //
 // Bounds: the metadata kernels by launch and load latency (two to four dependent
 // loads each: 512 rows over 100 000 pages 7.0, 4.3, 5.2 us for reserve's three
-// launches, 3.8 us for the release behind a window; 32 rows over 4000 pages 3.6,
-// 3.6, 5.8 and 2.8 us), the copies by HBM bandwidth.
+// launches, 3.8 us for the release behind a window; 32 rows over 4000 pages 4.9
+// and 5.7 us for its two, and 2.8 us), the copies by HBM bandwidth.
 #include <algorithm>
 
 #include "common.h"
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kPageThreads) share_pages_kernel(ShareArgs a) 
 // compact: the n live pages move to ids [0, n).  Those already there stay; the
 // k-th live page at or past n goes to the k-th free page below n, so no
 // destination is a source and one launch can copy them all.  4950 pages of 4 layers
-// x 32 KiB, 1.3 GB read and written: 256 us, 5.1 TB/s (a large copy moves 4.8);
+// x 32 KiB, 1.3 GB read and written: 246 us, 5.3 TB/s (a large copy moves 4.8);
 // the ranks before it 12 us.  Pages are copied layer by layer in units of 16 KiB, 4
 // loads of 16 bytes a thread at once, by one resident set of workgroups.
 struct CompactArgs {

@@ -28,9 +28,9 @@
 // A sliding window with sinks (WINDOW) only changes which pages a tile's KV loop
 // walks (window_tiles in plan.h) and the mask of its first and last KV tiles;
 // the tiles between run the step without a mask.  14 576 prompt tokens under a window
-// of 1023 (32/8 heads, D = 128) take 300 us: 231 GFLOP are seen, 0.77 PFLOP/s, and
-// 255 computed, 0.85 (18 KV tiles for the 1040 tokens that a row of a full q-tile
-// sees); a 512-token chunk under 4095, e4m3, 45 us and 9 us for its merge.
+// of 1023 (32/8 heads, D = 128) take 266 us: 231 GFLOP are seen, 0.87 PFLOP/s, and
+// 255 computed, 0.96 (18 KV tiles for the 1040 tokens that a row of a full q-tile
+// sees); a 512-token chunk under 4095, e4m3, 44 us and 9 us for its merge.
 //
 // Steps of few tiles (a 512-token chunk of a 32/8-head layer is 8 x 8
 // workgroups on 256 CUs) cut each tile's KV range into pieces, one workgroup
