@@ -577,3 +577,28 @@ def test_decode_on_a_device_that_is_not_current(gpu, kind, way, request):
     assert torch.cuda.current_device() == 0
     w = plan_decode(other, meta, heads, dtype, window, sinks, kind)
     check(*w.run(q, pool, return_lse=True), reference(meta, pool, scales, q, window, sinks))
+
+
+@pytest.mark.parametrize("heads,dtype,fp8", [
+    (HEADS[0], torch.float16, False), (HEADS[0], torch.bfloat16, True),
+    (HEADS[1], torch.bfloat16, False), (HEADS[1], torch.float16, True)])
+def test_prefill_of_more_than_two_rounds(gpu, heads, dtype, fp8):
+    """More q-tiles than twice those that run at once, whose list does not run in the order of
+    their lengths: every row is written, and as the other plan writes it."""
+    window, sinks = 127, 4
+    rng = np.random.default_rng(4)
+    tokens = 256 * heads[1] // heads[0]  # of a q-tile
+    tiles = 2 * (256 // heads[1]) + 9
+    chunks = [int(x) for x in rng.integers(1, tokens + 1, tiles)]
+    chunks[3] += 2 * tokens
+    computed = [int(x) for x in rng.integers(0, 300, tiles)]
+    meta, pool, scales, q = make(gpu, computed, chunks, heads, dtype, fp8, window, sinks, seed=3)
+    got = []
+    for device in (False, True):
+        out = torch.full_like(q.contiguous(), math.nan)
+        w = plan_prefill(gpu, meta, heads, dtype, window, sinks, device)
+        got.append(w.run(q, pool, kv_scales=scales, return_lse=True, out=out))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert bool(torch.isfinite(got[0][0]).all())
+    rows = sorted(set(rng.integers(0, meta.nnz, 60).tolist()) | {0, meta.nnz - 1})
+    check(*got[0], reference(meta, pool, scales, q, window, sinks, b_rows=set(rows)), rows)
