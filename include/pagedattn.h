@@ -209,7 +209,8 @@ int pagedattn_fork_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layers,
  *
  * pagedattn_reserve_pages: kv_lens[b] counts the step's new_lens[b] tokens (NULL:
  * one per sequence) already.  Every slot they open gets a free page (count
- * 1), lowest ids first in (row, slot) order.  A partial page that the tokens
+ * 1), lowest ids first in (row, slot) order; what it named before is not
+ * released.  A partial page that the tokens
  * continue and that others hold is forked first: a free page takes its rows in
  * every layer and its place in the table, and its count drops by one; of
  * several rows that continue one page, the last keeps it if nothing
@@ -229,8 +230,9 @@ int pagedattn_fork_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layers,
  * layer (those there already stay), with their counts and the entries that name
  * them; remap [num_pages] int32 gets each page's new id, -1 for free ones, for
  * tables kept elsewhere.
- * scratch: pagedattn_page_scratch_bytes device bytes, 256-byte aligned, for the
- * call alone. */
+ * Batches hold up to 65535 rows, and batch_size * (max_pages + 1) entries up to
+ * 2^31 - 1.  scratch: pagedattn_page_scratch_bytes device bytes, 256-byte aligned,
+ * for the call alone. */
 size_t pagedattn_page_scratch_bytes(int32_t num_pages, int32_t batch_size, int32_t max_pages);
 int pagedattn_reserve_pages(void* kv_pool, int32_t pool_dtype, int32_t num_layers,
                             int32_t num_pages, int32_t num_kv_heads, int32_t head_dim,

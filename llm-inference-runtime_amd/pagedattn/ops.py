@@ -23,7 +23,11 @@ Additions with no FlashInfer counterpart: ``build_paged_metadata`` (the
 step metadata built on the device), ``quantize_pages_e4m3``, the
 ``kv_scales`` argument for e4m3 pools with per-(page, K|V, kv-head) scales,
 ``append_paged_kv_cache_e4m3_amax`` (e4m3 append that maintains those
-scales as pages fill) and ``fork_pages`` (copy-on-write page fork).
+scales as pages fill), ``fork_pages`` (copy-on-write page fork), the page
+tables kept on the device (``reserve_pages``, ``release_pages``,
+``release_window_pages``, ``share_pages``, ``compact_pages``) and the positions
+of several axes (``apply_multi_axis_rope_inplace``,
+``multi_axis_rope_append_paged_kv_cache``).
 """
 
 from __future__ import annotations
