@@ -18,7 +18,8 @@ import pagedattn
 from pagedattn import llama as L
 from pagedattn.metadata import decode_metadata, prefill_metadata
 
-from paged_cases import i32, random_tables, require_shared_plans, strided_rows, workspace
+from paged_cases import (i32, random_tables, require_fixed_chunks, require_shared_plans,
+                         strided_rows, workspace)
 
 pytestmark = pytest.mark.gpu
 
@@ -169,6 +170,7 @@ def test_decode_many_sequences(gpu, kind):
     ref = reference(meta, pool, scales, q, window, sinks, b_rows=set(rows))
     check(out, lse, ref, rows)
     if kind == "device":
+        require_fixed_chunks()
         w.update_plan()
         again, lse2 = w.run(q, pool, return_lse=True)
         assert torch.equal(again, out) and torch.equal(lse2, lse)
@@ -190,6 +192,7 @@ def test_decode_long_window(gpu):
 @pytest.mark.parametrize("fp8", [False, True])
 def test_decode_fused_append_is_the_separate_calls(gpu, kind, batch, fp8):
     """RoPE + append + windowed attention in one call: the bits of the three."""
+    require_fixed_chunks()
     heads, window, sinks, dtype = HEADS[0], 100, 20, torch.bfloat16
     hq, hkv, d = heads
     lens = [LENS[i % len(LENS)] + 16 * (i % 5) for i in range(batch)]
@@ -531,6 +534,7 @@ def test_a_window_of_the_largest_size(gpu):
 @pytest.mark.parametrize("kind", ["host", "device"])
 def test_decode_by_the_general_path(gpu, kind, request):
     """The same bits as the extension's call, with RoPE and append and without."""
+    require_fixed_chunks()
     heads, dtype, window, sinks = HEADS[0], torch.float16, 60, 17
     meta, pool, _, q = make(gpu, [n - 1 for n in LENS], [1] * len(LENS), heads, dtype, False,
                             window, sinks, 1)
